@@ -94,10 +94,12 @@ def draw(rng):
     rows = rows if dtype == "bf16" else max(1, rows // 2)
     mask = rng.choice(["none", "tight", "loose", "mixed"])
     in_place = mask != "none" and rng.random() < 0.3
-    return {"kind": kind, "rows": rows, "vocab": vocab, "dtype": dtype,
-            "history": 0 if in_place else rng.choice([0, _log(rng, 16, 32768)]),
-            "lists": 0 if in_place else rng.choice([0, rng.randint(1, 128)]), "mask": mask, "in_place": in_place,
-            "frequency": rng.random() < 0.5, "shards": rng.choice([1, 1, 2, 8])}
+    history = 0 if in_place else rng.choice([0, _log(rng, 16, 32768)])
+    lists = 0 if in_place else rng.choice([0, rng.randint(1, 128)])
+    if mask == "none" and not history and not lists:  # a call with nothing to do is no case
+        history = _log(rng, 16, 32768)
+    return {"kind": kind, "rows": rows, "vocab": vocab, "dtype": dtype, "history": history, "lists": lists, "mask": mask,
+            "in_place": in_place, "frequency": rng.random() < 0.5, "shards": rng.choice([1, 1, 2, 8])}
 
 
 # ------------------------------------------------------------------ inputs --
