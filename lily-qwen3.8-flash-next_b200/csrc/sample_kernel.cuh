@@ -1081,10 +1081,12 @@ __device__ __forceinline__ void set_exact_threshold(SmemFixed *sm, uint32_t kth_
 }
 
 // At least k untouched logits have a raw key of `edge_key` or more: no logit
-// below that value can be among the best k (scaling keeps the order).
+// below that value can be among the best k (scaling keeps the order). An edge at or below
+// the key of -inf rejects nothing, and its value may be none: the keys below belong to
+// NaNs (a row of fewer finite logits than k ends up there: its k-th largest is -inf).
 __device__ __forceinline__ void set_raw_edge(SmemFixed *sm, uint32_t edge_key) {
     const RowCtx &c = sm->ctx;
-    if (edge_key == 0u) {
+    if (edge_key <= key_of(neg_inf())) {
         return;
     }
     float below = float_of_key(edge_key - 1u);
