@@ -61,7 +61,11 @@ enum lily_row_status {
     LILY_ROW_FORCED = 16     /* informational: the row returned its forced id */
 };
 
-enum lily_dtype { LILY_F32 = 0, LILY_BF16 = 1 };
+enum lily_dtype {
+    LILY_F32 = 0,
+    LILY_BF16 = 1,
+    LILY_E4M3 = 2 /* 8 bits; the calls of lily_layers.h only */
+};
 
 /*
  * src/kernels/sample.rs:19-31 SamplingParams, as a 40-byte POD (top_k as
@@ -331,6 +335,70 @@ int32_t lily_sample_batch_noalloc(void *stream, uint32_t vocab, const lily_sampl
 int32_t lily_argmax_batch(lily_sampler_t *h, void *stream, const void *logits,
                           uint32_t logits_dtype, uint64_t logits_ld, uint32_t rows,
                           uint32_t *out_ids);
+
+/* ---------------------------------------------- adjusted logits, masks -- */
+
+/*
+ * Biases, penalties, bans and grammar masks on logits, written out: what lily_sample_batch
+ * does to a row before it draws, for the paths whose draws take none of it (vocabulary shards,
+ * the rows of a speculative step, a head of the caller's own), and masks by bits, which no
+ * draw takes. Draw from the result with the penalties left out (lily_draft_params); a row then
+ * draws what lily_sample_batch draws with everything in the call, as long as `out` is F32.
+ *
+ *   l = logit; for the row's bias entries of that id, in list order: l += value
+ *   if penalties are on and count(id) > 0:
+ *       l = l > 0 ? l / repetition : l * repetition
+ *       l -= presence + frequency * count(id)
+ *   banned, or the id's bit in the row's mask is 0: l = -inf (whatever the logit was, NaN too)
+ *
+ * all in fp32, rounded once if `out` is BF16; the temperature stays with the draw. A row that
+ * is left with nothing is all -inf, which the draw reports (LILY_ROW_NONFINITE).
+ *
+ * The logits are those of the ids [first_id, first_id + handle vocab): 0 for a whole row, a
+ * shard's first id else. The ids of lists and masks are global; those outside the range have
+ * no effect. count(id) is the id's multiplicity in the row's history, or with `count_slots` its
+ * entry in the slot's histogram, which this call does not change.
+ *
+ * In place (`out` is `logits`, of the same type and pitch) only what changes is written. A row
+ * whose list is longer than max_history / max_list or its pitch, or whose device-resident
+ * params are invalid, is left as it was (in `out` too): status LILY_ROW_LIST / LILY_ROW_PARAMS,
+ * and the handle's sticky status. A row whose mask index is not below `masks` counts as LIST.
+ *
+ * Nothing of the handle is written but the status word: calls may overlap on the GPU.
+ */
+typedef struct lily_adjust_args {
+    uint32_t struct_size;        /* sizeof(lily_adjust_args_t) */
+    uint32_t rows;               /* 1..max_rows */
+    const void *logits;          /* [rows, logits_ld] of logits_dtype */
+    uint32_t logits_dtype;       /* LILY_F32 or LILY_BF16 */
+    uint32_t out_dtype;          /* logits_dtype, or LILY_F32 */
+    uint64_t logits_ld;          /* elements between rows (>= vocab) */
+    void *out;                   /* [rows, out_ld], or `logits`; else no overlap with it */
+    uint64_t out_ld;
+    const lily_sampling_params_t *params; /* [rows], its penalties; NULL: none */
+    uint32_t params_on_device;   /* 0: `params` is a HOST array */
+    uint32_t first_id;
+    const uint32_t *history_ids; /* the lists as in lily_sample_args_t */
+    const uint32_t *history_len;
+    uint64_t history_ld;
+    const uint32_t *bias_ids;
+    const float *bias_vals;
+    const uint32_t *bias_len;
+    uint64_t bias_ld;
+    const uint32_t *ban_ids;
+    const uint32_t *ban_len;
+    uint64_t ban_ld;
+    const uint32_t *count_slots; /* HOST [rows] histogram slots, or NULL; first_id 0 only */
+    const uint32_t *mask;        /* [masks, mask_ld] words or NULL: bit i % 32 of word i / 32 set = id i may
+                                    be drawn; words up to id first_id + vocab - 1 are read */
+    uint64_t mask_ld;            /* words between masks */
+    const int32_t *mask_rows;    /* [rows] a row's mask, < 0 = none; NULL: row r has mask r */
+    uint32_t masks;              /* how many there are */
+    uint32_t reserved;
+    uint32_t *out_status;        /* [rows] enum lily_row_status, or NULL */
+} lily_adjust_args_t;
+
+int32_t lily_adjust_logits(lily_sampler_t *h, void *stream, const lily_adjust_args_t *args);
 
 /* ------------------------------------------------------------ speculation -- */
 

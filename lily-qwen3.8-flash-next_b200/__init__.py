@@ -1,4 +1,4 @@
-"""Python binding of the B200 token sampler's C ABI (include/lily_sampler.h).
+"""Python binding of the B200 token sampler's C ABI (include/lily_sampler.h, include/lily_layers.h).
 
 The names mirror the reference's sampler interface (paths relative to the
 reference project): `SamplingParams` (src/kernels/sample.rs:19-95),
@@ -21,7 +21,7 @@ LIB_PATH = os.path.join(_HERE, "liblily_sampler.so")
 CALLS_PATH = os.path.join(_HERE, "_lily_calls.so")
 
 K_CAP = 1024
-F32, BF16 = 0, 1
+F32, BF16, E4M3 = 0, 1, 2
 SPEC_REJECTION, SPEC_GREEDY_MATCH = 0, 1
 FLAG_COUNTS_TABLE = 1
 FLAG_PHASE_CLOCKS = 2
@@ -135,6 +135,50 @@ class SpecArgs(C.Structure):
     ]
 
 
+class AdjustArgs(C.Structure):
+    """lily_adjust_args_t: biases, penalties, bans and masks written onto logits."""
+
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("rows", C.c_uint32),
+        ("logits", _vp), ("logits_dtype", C.c_uint32), ("out_dtype", C.c_uint32), ("logits_ld", C.c_uint64),
+        ("out", _vp), ("out_ld", C.c_uint64),
+        ("params", _vp), ("params_on_device", C.c_uint32), ("first_id", C.c_uint32),
+        ("history_ids", _u32p), ("history_len", _u32p), ("history_ld", C.c_uint64),
+        ("bias_ids", _u32p), ("bias_vals", _f32p), ("bias_len", _u32p), ("bias_ld", C.c_uint64),
+        ("ban_ids", _u32p), ("ban_len", _u32p), ("ban_ld", C.c_uint64),
+        ("count_slots", _u32p),
+        ("mask", _u32p), ("mask_ld", C.c_uint64), ("mask_rows", _i32p), ("masks", C.c_uint32),
+        ("reserved", C.c_uint32), ("out_status", _u32p),
+    ]
+
+
+class NormArgs(C.Structure):
+    """lily_norm_args_t (include/lily_layers.h)."""
+
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("tokens", C.c_uint32), ("hidden", C.c_uint32), ("dtype", C.c_uint32),
+        ("x", _vp), ("x_ld", C.c_uint64), ("residual", _vp), ("residual_ld", C.c_uint64),
+        ("residual_out", _vp), ("residual_out_ld", C.c_uint64),
+        ("weight", _vp), ("weight_dtype", C.c_uint32), ("out_dtype", C.c_uint32),
+        ("out", _vp), ("out_ld", C.c_uint64), ("out_scales", _f32p), ("eps", C.c_float), ("weight_offset", C.c_float),
+    ]
+
+
+class LinearArgs(C.Structure):
+    """lily_linear_args_t (include/lily_layers.h)."""
+
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("tokens", C.c_uint32), ("columns", C.c_uint32), ("outputs", C.c_uint32),
+        ("dtype", C.c_uint32), ("out_dtype", C.c_uint32),
+        ("a", _vp), ("a_ld", C.c_uint64), ("weight", _vp), ("weight_ld", C.c_uint64),
+        ("a_scales", _f32p), ("weight_scales", _f32p),
+        ("bias", _vp), ("bias_dtype", C.c_uint32), ("activation", C.c_uint32),
+        ("residual", _vp), ("residual_ld", C.c_uint64), ("out", _vp), ("out_ld", C.c_uint64),
+    ]
+
+
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
+
 _lib = None
 
 
@@ -218,6 +262,9 @@ def lib():
                                          C.c_uint32, C.c_uint32]
         L.lily_merge_draw_peer.argtypes = [C.c_void_p, C.c_void_p, C.POINTER(PeerExchangeStruct), C.c_void_p,
                                            C.c_uint32, C.POINTER(SampleArgs), C.c_void_p]
+        L.lily_adjust_logits.argtypes = [C.c_void_p, C.c_void_p, C.POINTER(AdjustArgs)]
+        L.lily_add_rms_norm.argtypes = [C.c_void_p, C.c_void_p, C.POINTER(NormArgs)]
+        L.lily_linear.argtypes = [C.c_void_p, C.c_void_p, C.POINTER(LinearArgs)]
         _lib = L
     return _lib
 
@@ -324,6 +371,41 @@ def _stream_ptr(stream) -> int:
     return stream.cuda_stream
 
 
+class _Rows:
+    """A tensor as a call around the head takes it: on the handle's device, one- or
+    two-dimensional, its rows contiguous and any distance apart."""
+
+    def __init__(self, name, t, device, types, rows=None, columns=None):
+        self.p, self.ld, self.rows, self.columns, self.dtype = None, 0, 0, 0, 0
+        if t is None:
+            return
+        import torch
+
+        codes = {torch.float32: F32, torch.bfloat16: BF16, torch.float8_e4m3fn: E4M3}
+        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.device.index != device:
+            raise LilyError(ERR_ARG, f"{name} must be a tensor on the handle's device, cuda:{device}")
+        if t.dtype not in types:
+            raise LilyError(ERR_ARG, f"{name} is {t.dtype}: it must be one of {', '.join(str(x) for x in types)}")
+        if t.dim() not in (1, 2) or t.numel() == 0:
+            raise LilyError(ERR_ARG, f"{name} must be [n] or [rows, n], and not empty")
+        self.rows, self.columns = (t.shape[0] if t.dim() == 2 else 1), t.shape[-1]
+        if (self.columns > 1 and t.stride(-1) != 1) or (self.rows > 1 and t.stride(0) < self.columns):
+            raise LilyError(ERR_ARG, f"the rows of {name} must be contiguous and not overlap")
+        for is_, want in ((self.rows, rows), (self.columns, columns)):
+            if want is not None and is_ != want:
+                raise LilyError(ERR_ARG, f"{name} is {list(t.shape)}: it does not go with the other arguments")
+        self.p, self.dtype = t.data_ptr(), codes.get(t.dtype, 0)
+        self.ld = t.stride(0) if self.rows > 1 else self.columns
+
+
+def _values(name, t, device, types, n):
+    """The address of n values in a row (of one row, or of rows that follow one another)."""
+    r = _Rows(name, t, device, types)
+    if r.p is not None and (r.rows * r.columns != n or (r.rows > 1 and r.ld != r.columns)):
+        raise LilyError(ERR_ARG, f"{name} must be {n} values, contiguous")
+    return r.p
+
+
 class SamplerScratch:
     """Per-engine sampler state for one vocabulary (src/kernels/sample.rs:115-179),
     for up to `max_rows` rows per call."""
@@ -347,6 +429,7 @@ class SamplerScratch:
             raise LilyError(st, "lily_sampler_create failed (is a CUDA device present?)")
         self._calls = calls()
         self._addr = self._h.value
+        self._vocab = vocab
 
     def close(self):
         if getattr(self, "_h", None) is not None and self._h:
@@ -613,6 +696,129 @@ class SamplerScratch:
             a.kept_ld = _ld(kept_ids)
         self._check(lib().lily_merge_draw_peer(self._h, _stream_ptr(stream), C.byref(exchange), _ptr(records),
                                                step, C.byref(a), _ptr(out_lse)))
+
+    # -- around the head: the norm before it, products, adjusted logits
+    def _stream_here(self, stream) -> int:
+        import torch
+
+        return (torch.cuda.current_stream(self.device) if stream is None else stream).cuda_stream
+
+    def add_rms_norm(self, x, weight, out, *, residual=None, residual_out=None, out_scales=None, eps: float = 1e-6,
+                     weight_offset: float = 0.0, stream=None):
+        """lily_add_rms_norm: `out` [tokens, hidden] = the root-mean-square norm of x + residual, times
+        weight_offset + weight. x, residual and residual_out (the sum, rounded) are F32 or BF16; out is F32,
+        BF16, or torch.float8_e4m3fn with f32 `out_scales` [tokens]. out and residual_out may be x or residual."""
+        st = self._calls.add_rms_norm(self._addr, self.device, stream, x, weight, out, residual, residual_out,
+                                      out_scales, eps, weight_offset)
+        if st is None:
+            import torch
+
+            wide, dev = (torch.float32, torch.bfloat16), self.device
+            x_ = _Rows("x", x, dev, wide)
+            size = (x_.rows, x_.columns)
+            w_ = _Rows("weight", weight, dev, wide, 1, x_.columns)
+            o_ = _Rows("out", out, dev, (*wide, torch.float8_e4m3fn), *size)
+            r_, s_ = (_Rows(n, t, dev, (x.dtype,), *size) for n, t in (("residual", residual),
+                                                                       ("residual_out", residual_out)))
+            scales = _values("out_scales", out_scales, dev, (torch.float32,), x_.rows)
+            a = NormArgs(C.sizeof(NormArgs), x_.rows, x_.columns, x_.dtype, x_.p, x_.ld, r_.p, r_.ld, s_.p, s_.ld,
+                         w_.p, w_.dtype, o_.dtype, o_.p, o_.ld, scales, eps, weight_offset)
+            st = lib().lily_add_rms_norm(self._h, self._stream_here(stream), C.byref(a))
+        if st:
+            self._check(st)
+
+    def linear(self, a, weight, out, *, a_scales=None, weight_scales=None, bias=None, activation: str = "none",
+               residual=None, stream=None):
+        """lily_linear: `out` [tokens, outputs] = act(a @ weight^T + bias) + residual. a [tokens, columns] and
+        weight [outputs, columns] are both BF16, or both torch.float8_e4m3fn with f32 a_scales [tokens] and
+        weight_scales [outputs]; out and residual are F32 or BF16. activation: one of ACTIVATIONS."""
+        act = ACTIVATIONS.get(activation)
+        if act is None:
+            raise LilyError(ERR_ARG, f"activation {activation!r}: it must be one of {', '.join(ACTIVATIONS)}")
+        st = self._calls.linear(self._addr, self.device, stream, a, weight, out, a_scales, weight_scales, bias, act,
+                                residual)
+        if st is None:
+            import torch
+
+            wide, dev = (torch.float32, torch.bfloat16), self.device
+            a_ = _Rows("a", a, dev, (torch.bfloat16, torch.float8_e4m3fn))
+            w_ = _Rows("weight", weight, dev, (a.dtype,), None, a_.columns)
+            o_ = _Rows("out", out, dev, wide, a_.rows, w_.rows)
+            r_ = _Rows("residual", residual, dev, (out.dtype,), a_.rows, w_.rows)
+            b_ = _Rows("bias", bias, dev, wide, 1, w_.rows)
+            args = LinearArgs(C.sizeof(LinearArgs), a_.rows, a_.columns, w_.rows, a_.dtype, o_.dtype, a_.p, a_.ld, w_.p,
+                              w_.ld, _values("a_scales", a_scales, dev, (torch.float32,), a_.rows),
+                              _values("weight_scales", weight_scales, dev, (torch.float32,), w_.rows),
+                              b_.p, b_.dtype, act, r_.p, r_.ld, o_.p, o_.ld)
+            st = lib().lily_linear(self._h, self._stream_here(stream), C.byref(args))
+        if st:
+            self._check(st)
+
+    def adjust_logits(self, logits, params=None, out=None, *, stream=None, **kw):
+        """lily_adjust_logits: biases, the penalties of `params`, bans and masks onto `logits` [rows, vocab], in
+        place or into `out`. Keywords: history_ids / history_len, bias_ids / bias_vals / bias_len, ban_ids /
+        ban_len and count_slots as in sample_batch, params_on_device, mask (int32 words, bit i % 32 of word
+        i / 32 set = id i may be drawn; [masks, words]) with mask_rows (a row's mask, < 0 none), first_id (of
+        a vocabulary shard), out_status. Draw from the result with draft_params(params)."""
+        st = self._calls.adjust_logits(self._addr, self.device, stream, self._vocab, logits, params, out, kw)
+        if st is None:
+            st = self._adjust_logits(logits, params, out, stream, **kw)
+        if st:
+            self._check(st)
+
+    def _adjust_logits(self, logits, params, out, stream, *, history_ids=None, history_len=None, bias_ids=None,
+                       bias_vals=None, bias_len=None, ban_ids=None, ban_len=None, count_slots=None,
+                       params_on_device=False, mask=None, mask_rows=None, first_id=0, out_status=None):
+        import torch
+
+        dev, wide = self.device, (torch.float32, torch.bfloat16)
+        word = (torch.int32, torch.uint32)
+        l_ = _Rows("logits", logits, dev, wide, None, self.vocab())
+        rows = l_.rows
+        o_ = l_ if out is None else _Rows("out", out, dev, wide, rows, self.vocab())
+        a = AdjustArgs()
+        a.struct_size, a.rows = C.sizeof(AdjustArgs), rows
+        a.logits, a.logits_dtype, a.logits_ld = l_.p, l_.dtype, l_.ld
+        a.out, a.out_dtype, a.out_ld = o_.p, o_.dtype, o_.ld
+        if params_on_device:
+            a.params_on_device = 1
+            a.params = _values("params", params, dev, (torch.uint8,), rows * C.sizeof(SamplingParams))
+        elif params is not None:
+            if len(params) != rows:
+                raise LilyError(ERR_ARG, f"{len(params)} params for {rows} rows")
+            arr = (SamplingParams * rows)(*params)
+            a.params = C.cast(arr, C.c_void_p)
+        for name, ids, length in (("history", history_ids, history_len), ("bias", bias_ids, bias_len),
+                                  ("ban", ban_ids, ban_len)):
+            if (ids is None) != (length is None):
+                raise LilyError(ERR_ARG, f"{name}_ids and {name}_len go together")
+            if ids is not None and ids.numel() == 0:
+                continue  # (lists that can hold nothing)
+            r = _Rows(f"{name}_ids", ids, dev, word, rows)
+            if r.rows > 1 and r.ld != r.columns:
+                raise LilyError(ERR_ARG, f"{name}_ids must be contiguous")
+            setattr(a, f"{name}_ids", r.p)
+            setattr(a, f"{name}_ld", r.ld)
+            setattr(a, f"{name}_len", _values(f"{name}_len", length, dev, word, rows))
+        if (bias_ids is None) != (bias_vals is None):
+            raise LilyError(ERR_ARG, "bias_ids and bias_vals go together")
+        if a.bias_ids:
+            a.bias_vals = _values("bias_vals", bias_vals, dev, (torch.float32,), rows * a.bias_ld)
+        if count_slots is not None:
+            if len(count_slots) != rows:
+                raise LilyError(ERR_ARG, f"{len(count_slots)} slots for {rows} rows")
+            carr = (C.c_uint32 * rows)(*[int(s) for s in count_slots])
+            a.count_slots = C.cast(carr, C.c_void_p)
+        if not 0 <= first_id <= 0xFFFFFFFF:
+            raise LilyError(ERR_ARG, "first_id must be an id")
+        a.first_id = first_id
+        m_ = _Rows("mask", mask, dev, word)
+        if m_.p is not None and m_.columns * 32 < first_id + self.vocab():
+            raise LilyError(ERR_ARG, "mask has fewer bits than there are ids")
+        a.mask, a.mask_ld, a.masks = m_.p, m_.ld, m_.rows
+        a.mask_rows = _values("mask_rows", mask_rows, dev, (torch.int32,), rows)
+        a.out_status = _values("out_status", out_status, dev, word, rows)
+        return lib().lily_adjust_logits(self._h, self._stream_here(stream), C.byref(a))
 
     def argmax_batch(self, logits, out_ids, stream=None):
         """src/kernels/elementwise.rs:297-308 argmax_f32 for each row."""

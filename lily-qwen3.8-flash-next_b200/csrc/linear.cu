@@ -1,0 +1,483 @@
+// A matrix product with its bias, activation and residual (lily_linear, include/lily_layers.h):
+//
+//   out[t, n] = act(sa[t] * sw[n] * sum_k a[t, k] * w[n, k] + bias[n]) + residual[t, n]
+//
+// The multiplier's M side takes the weights (128 outputs a tile) and its N side the tokens, so
+// that few tokens waste nothing: a step's time is its weights' stream. A lane of tensor memory is
+// then an output and a column a token: an epilogue thread owns one output (its scale and bias are two
+// registers), and a warp writes 32 neighbouring outputs of a token at a time.
+#include <cuda_bf16.h>
+
+#include <algorithm>
+#include <atomic>
+#include <cstring>
+
+#include "../../include/lily_layers.h"
+#include "handle.cuh"
+#include "lmhead_args.cuh"
+#include "tc.cuh"
+
+namespace {
+
+using namespace lily_host;
+using namespace lily_tc;
+
+constexpr uint32_t TILE_M = 128;       // outputs of a tile
+constexpr uint32_t BLOCK_BYTES = 128;  // of a row's columns, a step of the pipeline: 64 bf16, 128 e4m3
+constexpr uint32_t A_STAGE = TILE_M * BLOCK_BYTES;
+constexpr uint32_t FULL = 0xFFFFFFFFu;
+
+struct LinearArgs {
+    CUtensorMap w_map;  // [outputs, columns], boxes of 128 rows x 128 bytes, 128-byte swizzle
+    CUtensorMap a_map;  // [tokens, columns], boxes of a token tile x 128 bytes
+    const float *a_scales, *w_scales;
+    const void *bias, *residual;
+    void *out;
+    uint64_t residual_ld, out_ld;
+    uint32_t tokens, outputs;
+    uint32_t blocks;        // steps of BLOCK_BYTES in a row
+    uint32_t token_tiles;
+    uint32_t out_f32, bias_f32, activation;
+    uint32_t *status_word;
+    uint64_t wait_ns;
+    uint32_t lost_stage;    // test hook: the first block leaves out the copies of this step (~0: none)
+};
+
+__device__ __forceinline__ float activated(float v, uint32_t activation) {
+    switch (activation) {
+        case LILY_ACT_RELU:
+            return v < 0.0f ? 0.0f : v;  // (a NaN stays)
+        case LILY_ACT_SILU:
+            return v / (1.0f + expf(-v));
+        case LILY_ACT_GELU:
+            return 0.5f * v * (1.0f + erff(v * 0.70710678f));
+        case LILY_ACT_GELU_TANH:
+            return 0.5f * v * (1.0f + tanhf(0.79788456f * (v + 0.044715f * v * v * v)));
+        default:
+            return v;
+    }
+}
+
+// What a thread of the epilogue knows of its output n.
+struct Output {
+    float scale, bias;
+    bool live;
+};
+
+__device__ __forceinline__ Output output_of(const LinearArgs &a, uint32_t n) {
+    Output o = {1.0f, 0.0f, n < a.outputs};
+    if (o.live && a.w_scales != nullptr) {
+        o.scale = __ldg(a.w_scales + n);
+    }
+    if (o.live && a.bias != nullptr) {
+        o.bias = a.bias_f32 ? __ldg(static_cast<const float *>(a.bias) + n)
+                            : __bfloat162float(static_cast<const __nv_bfloat16 *>(a.bias)[n]);
+    }
+    return o;
+}
+
+__device__ __forceinline__ float residual_at(const LinearArgs &a, uint32_t t, uint32_t n) {
+    const uint64_t at = (uint64_t)t * a.residual_ld + n;
+    return a.out_f32 ? static_cast<const float *>(a.residual)[at]
+                     : __bfloat162float(static_cast<const __nv_bfloat16 *>(a.residual)[at]);
+}
+
+__device__ __forceinline__ void finish(const LinearArgs &a, const Output &o, uint32_t t, uint32_t n, float sum,
+                                       float residual) {
+    float v = a.a_scales != nullptr ? sum * (__ldg(a.a_scales + t) * o.scale) : sum;
+    v = activated(v + o.bias, a.activation) + residual;
+    const uint64_t at = (uint64_t)t * a.out_ld + n;
+    if (a.out_f32) {
+        static_cast<float *>(a.out)[at] = v;
+    } else {
+        static_cast<__nv_bfloat16 *>(a.out)[at] = __float2bfloat16_rn(v);
+    }
+}
+
+// D binary32; A and B both bf16 (kind::f16) or both e4m3 (kind::f8f6f4), both K-major.
+template <bool E4M3>
+__device__ __forceinline__ uint32_t product_desc(uint32_t m, uint32_t n) {
+    return (1u << 4) | (E4M3 ? 0u : (1u << 7) | (1u << 10)) | ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+
+// D[tmem] (+)= A[smem] * B[smem]^T over 32 bytes of columns.
+template <bool E4M3>
+__device__ __forceinline__ void mma_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    if (E4M3) {
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+            ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+            : "memory");
+    } else {
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+            ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+            : "memory");
+    }
+}
+
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+// ------------------------------------------------------------------ few tokens --
+//
+// One tile of 128 outputs x N tokens per cluster; the cluster's blocks share the columns out
+// evenly. Each sums its share in tensor memory, then sends every token's column of sums to the
+// block that finishes that token, which adds the shares up in the blocks' order.
+//
+// A block's warps: 0 asks for the copies, 1 issues the multiplies, 2 to 5 are the epilogue.
+template <uint32_t N>
+struct Few {
+    static constexpr uint32_t THREADS = 192;
+    static constexpr uint32_t B_STAGE = N * BLOCK_BYTES;
+    static constexpr uint32_t STAGE = A_STAGE + B_STAGE;
+    static constexpr uint32_t PART_BYTES = N * TILE_M * 4u;
+    // Two blocks on an SM up to 64 tokens, else one.
+    static constexpr uint32_t STAGES = N == 16u ? 5u : N == 32u ? 4u : N == 64u ? 3u : 4u;
+    // Sums of successive steps go into accumulators in turn: shorter chains of additions.
+    static constexpr uint32_t ACCS = N <= 64u ? 4u : 2u;
+    static constexpr uint32_t COLS = ACCS * N < 32u ? 32u : ACCS * N;
+    static constexpr uint32_t PART = STAGES * STAGE;
+    static constexpr uint32_t BARS = PART + PART_BYTES;
+    static constexpr uint32_t EMPTY = BARS + 8u * STAGES;
+    static constexpr uint32_t FINAL = EMPTY + 8u * STAGES;
+    static constexpr uint32_t TMEM_ADDR = FINAL + 8u;
+    static constexpr uint32_t ABORT = TMEM_ADDR + 4u;
+    static constexpr uint32_t BYTES = ABORT + 4u + 1024u;
+    static_assert(BYTES <= 227u * 1024u && BYTES > 76u * 1024u, "at most two blocks on an SM");
+    static_assert(COLS <= 256u && (COLS & (COLS - 1u)) == 0u, "tensor memory of two blocks on an SM");
+};
+
+template <uint32_t N, bool E4M3>
+__global__ void __launch_bounds__(192) linear_few_kernel(const __grid_constant__ LinearArgs a) {
+    using S = Few<N>;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t *smem = smem_raw + (base - smem_u32(smem_raw));
+    volatile uint32_t *abort_word = reinterpret_cast<volatile uint32_t *>(smem + S::ABORT);
+    const uint32_t tid = threadIdx.x, warp = __shfl_sync(FULL, tid / 32u, 0), lane = tid % 32u;
+    uint32_t rank, shares;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(shares));
+    const uint32_t tile = blockIdx.x / shares;
+    const uint32_t token0 = tile % a.token_tiles * N, output0 = tile / a.token_tiles * TILE_M;
+    const uint32_t block0 = (uint32_t)((uint64_t)a.blocks * rank / shares);
+    const uint32_t steps = (uint32_t)((uint64_t)a.blocks * (rank + 1u) / shares) - block0;
+
+    if (tid == 0) {
+        for (uint32_t s = 0; s < S::STAGES; ++s) {
+            mbar_init(base + S::BARS + 8 * s, 1);
+            mbar_init(base + S::EMPTY + 8 * s, 1);
+        }
+        mbar_init(base + S::FINAL, 1);
+        *abort_word = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1u) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + S::TMEM_ADDR),
+                     "r"(S::COLS)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(smem + S::TMEM_ADDR);
+    if (shares > 1u) {
+        cluster_arrive();  // (this block has begun: the others may write into its shared memory)
+    }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    // (Behind the allocation: a block of the next launch that held tensor memory before all of this
+    // launch's have theirs would wait for them, and they for it.)
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+    if (warp == 0u) {
+        if (lane == 0u) {
+            uint32_t asked = 0, parity = 0;
+            for (uint32_t i = 0; i < steps; ++i) {
+                const uint32_t s = i % S::STAGES, use = i / S::STAGES;
+                if (mbar_wait(base + S::EMPTY + 8 * s, (use & 1u) ^ 1u, abort_word, a.wait_ns)) {
+                    break;
+                }
+                const uint32_t bar = base + S::BARS + 8 * s, to = base + s * S::STAGE;
+                const int32_t x = (int32_t)((block0 + i) * (E4M3 ? BLOCK_BYTES : BLOCK_BYTES / 2u));
+                if (i == a.lost_stage && blockIdx.x == 0u) {
+                    continue;  // (test hook: the stage never fills)
+                }
+                asked |= 1u << s;
+                parity = (parity & ~(1u << s)) | (use & 1u) << s;
+                mbar_expect_tx(bar, S::STAGE);
+                tma_load_2d(to, &a.w_map, bar, x, (int32_t)output0);
+                tma_load_2d(to + A_STAGE, &a.a_map, bar, x, (int32_t)token0);
+            }
+            if (*abort_word) {  // the copies asked for land in this block's shared memory: it stays until they have
+                for (uint32_t s = 0; s < S::STAGES; ++s) {
+                    if (asked >> s & 1u) {
+                        mbar_drain(base + S::BARS + 8 * s, parity >> s & 1u, a.wait_ns);
+                    }
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1u) {
+        const bool leader = elect_one();
+        const uint32_t idesc = product_desc<E4M3>(TILE_M, N);
+        for (uint32_t i = 0; i < steps; ++i) {
+            const uint32_t s = i % S::STAGES;
+            if (warp_wait(base + S::BARS + 8 * s, i / S::STAGES & 1u, abort_word, a.wait_ns)) {
+                break;
+            }
+            tc_fence_after();
+            if (leader) {
+                const uint64_t adesc = operand_desc(base + s * S::STAGE), bdesc = operand_desc(base + s * S::STAGE + A_STAGE);
+#pragma unroll
+                for (uint32_t k = 0; k < 4u; ++k) {
+                    mma_ss<E4M3>(tmem + i % S::ACCS * N, adesc + 2u * k, bdesc + 2u * k, idesc, i >= S::ACCS || k > 0u);
+                }
+                mma_commit(base + S::EMPTY + 8 * s);
+            }
+            __syncwarp();
+        }
+        if (leader) {
+            mma_commit(base + S::FINAL);
+            mbar_drain(base + S::FINAL, 0u, a.wait_ns);  // (nothing is freed under a multiply, on any way out)
+        }
+        __syncwarp();
+    }
+
+    const uint32_t quad = warp % 4u, row = quad * 32u + lane;  // the epilogue's lanes of tensor memory
+    const uint32_t n = output0 + row, live = min(N, a.tokens - token0);
+    const uint32_t accs = min(S::ACCS, steps), from = tmem + (quad * 32u << 16);
+    // Sixteen tokens' sums of this thread's output.
+    const auto sums_of = [&](uint32_t c, float (&v)[16]) {
+        uint32_t q[16];
+        tmem_ld16(from + c, q);
+        tmem_ld_wait();
+#pragma unroll
+        for (uint32_t j = 0; j < 16u; ++j) {
+            v[j] = __uint_as_float(q[j]);
+        }
+        for (uint32_t k = 1; k < accs; ++k) {
+            tmem_ld16(from + k * N + c, q);
+            tmem_ld_wait();
+#pragma unroll
+            for (uint32_t j = 0; j < 16u; ++j) {
+                v[j] += __uint_as_float(q[j]);
+            }
+        }
+    };
+    if (shares == 1u) {
+        if (warp >= 2u) {
+            const Output o = output_of(a, n);
+            warp_wait(base + S::FINAL, 0u, abort_word, a.wait_ns);
+            tc_fence_after();
+            for (uint32_t c = 0; c < live; c += 16u) {
+                float v[16], r[16];
+#pragma unroll
+                for (uint32_t j = 0; j < 16u; ++j) {
+                    r[j] = a.residual != nullptr && o.live && c + j < live ? residual_at(a, token0 + c + j, n) : 0.0f;
+                }
+                sums_of(c, v);
+#pragma unroll
+                for (uint32_t j = 0; j < 16u; ++j) {
+                    if (o.live && c + j < live) {
+                        finish(a, o, token0 + c + j, n, v[j], r[j]);
+                    }
+                }
+            }
+        }
+    } else {
+        // Token c is finished by block c / per; its sums lie there at [share][c % per][output].
+        const uint32_t per = N / shares;
+        cluster_wait();
+        if (warp >= 2u) {
+            warp_wait(base + S::FINAL, 0u, abort_word, a.wait_ns);
+            tc_fence_after();
+            for (uint32_t c = 0; c < live; c += 16u) {
+                float v[16];
+                sums_of(c, v);
+#pragma unroll
+                for (uint32_t j = 0; j < 16u; ++j) {
+                    if (c + j < live) {
+                        const uint32_t here = base + S::PART + ((rank * per + (c + j) % per) * TILE_M + row) * 4u;
+                        uint32_t there;
+                        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(here), "r"((c + j) / per));
+                        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(there), "f"(v[j]) : "memory");
+                    }
+                }
+            }
+        }
+        __syncwarp();
+        cluster_arrive();
+        cluster_wait();
+        if (warp >= 2u) {
+            const Output o = output_of(a, n);
+            const float *part = reinterpret_cast<const float *>(smem + S::PART) + row;
+            for (uint32_t c = rank * per; c < min(live, (rank + 1u) * per); ++c) {
+                const float r = a.residual != nullptr && o.live ? residual_at(a, token0 + c, n) : 0.0f;
+                float v = part[c % per * TILE_M];
+                for (uint32_t k = 1; k < shares; ++k) {
+                    v += part[(k * per + c % per) * TILE_M];
+                }
+                if (o.live) {
+                    finish(a, o, token0 + c, n, v, r);
+                }
+            }
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 1u) {
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::COLS) : "memory");
+    }
+    if (tid == 0 && *abort_word) {
+        atomicOr(a.status_word, 1u << lily_head::STATUS_TIMEOUT_BIT);
+    }
+}
+
+template <typename Kernel>
+cudaError_t set_up(Kernel kernel, uint32_t bytes, std::atomic<uint64_t> &ready) {
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    const uint64_t bit = 1ull << (device & 63);  // (bit d: device d has seen the set-up)
+    if (e == cudaSuccess && !(ready.load(std::memory_order_relaxed) & bit)) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+        ready.fetch_or(e == cudaSuccess ? bit : 0u, std::memory_order_relaxed);
+    }
+    return e;
+}
+
+template <uint32_t N, bool E4M3>
+cudaError_t launch_few(const LinearArgs &a, uint32_t tiles, uint32_t shares, cudaStream_t stream) {
+    static std::atomic<uint64_t> ready{0};
+    const cudaError_t e = set_up(linear_few_kernel<N, E4M3>, Few<N>::BYTES, ready);
+    if (e != cudaSuccess) {
+        return e;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(tiles * shares, 1, 1);
+    cfg.blockDim = dim3(Few<N>::THREADS, 1, 1);
+    cfg.dynamicSmemBytes = Few<N>::BYTES;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = shares;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, linear_few_kernel<N, E4M3>, a);
+}
+
+template <bool E4M3>
+cudaError_t few_by_tokens(const LinearArgs &a, uint32_t n, uint32_t tiles, uint32_t shares, cudaStream_t stream) {
+    return n == 16u   ? launch_few<16, E4M3>(a, tiles, shares, stream)
+           : n == 32u ? launch_few<32, E4M3>(a, tiles, shares, stream)
+           : n == 64u ? launch_few<64, E4M3>(a, tiles, shares, stream)
+                      : launch_few<128, E4M3>(a, tiles, shares, stream);
+}
+
+bool encode_rows(CUtensorMap *map, const void *p, uint64_t ld, uint32_t rows, uint32_t columns, uint32_t dtype,
+                 uint32_t box_rows) {
+    const uint32_t size = dtype == LILY_BF16 ? 2u : 1u;
+    const cuuint64_t dims[2] = {columns, rows};
+    // (The pitch of a single row is never used, but has to be in order.)
+    const cuuint64_t strides[1] = {rows > 1u ? ld * size : ((uint64_t)columns * size + 15u) & ~uint64_t(15)};
+    const cuuint32_t box[2] = {BLOCK_BYTES / size, box_rows};
+    const cuuint32_t estr[2] = {1, 1};
+    return tensor_map_encoder()(map, size == 2u ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2,
+                                const_cast<void *>(p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace
+
+extern "C" int32_t lily_linear(lily_sampler_t *h, void *stream_, const lily_linear_args_t *args) {
+    const int32_t st = check_handle(h);
+    if (st != LILY_OK) {
+        return st;
+    }
+    if (args == nullptr || args->struct_size != sizeof(lily_linear_args_t)) {
+        return fail(h, LILY_ERR_ARG, "args is null or of another ABI version");
+    }
+    const lily_linear_args_t &g = *args;
+    constexpr uint32_t MOST = 1u << 30;  // (coordinates of copies are 32 bits, signed)
+    if (g.tokens == 0u || g.columns == 0u || g.outputs == 0u || g.tokens > MOST || g.columns > MOST || g.outputs > MOST) {
+        return fail(h, LILY_ERR_CAPACITY, "tokens, columns and outputs must be 1..2^30");
+    }
+    if (g.a == nullptr || g.weight == nullptr || g.out == nullptr) {
+        return fail(h, LILY_ERR_ARG, "a, weight and out must be set");
+    }
+    if ((g.dtype != LILY_BF16 && g.dtype != LILY_E4M3) || g.out_dtype > LILY_BF16 || g.bias_dtype > LILY_BF16 ||
+        g.activation > LILY_ACT_GELU_TANH) {
+        return fail(h, LILY_ERR_ARG, "a and weight are BF16 or E4M3, out and bias F32 or BF16, activation one of the five");
+    }
+    const bool e4m3 = g.dtype == LILY_E4M3;
+    if ((g.a_scales != nullptr) != e4m3 || (g.weight_scales != nullptr) != e4m3) {
+        return fail(h, LILY_ERR_ARG, "a_scales and weight_scales go with E4M3, and only with it");
+    }
+    if (g.a_ld < g.columns || g.weight_ld < g.columns || g.out_ld < g.outputs ||
+        (g.residual != nullptr && g.residual_ld < g.outputs)) {
+        return fail(h, LILY_ERR_ARG, "a row pitch is smaller than its row");
+    }
+    const uint32_t size = e4m3 ? 1u : 2u, out_size = g.out_dtype == LILY_F32 ? 4u : 2u;
+    if (reinterpret_cast<uintptr_t>(g.a) % 16u || reinterpret_cast<uintptr_t>(g.weight) % 16u ||
+        (g.tokens > 1u && g.a_ld * size % 16u) || (g.outputs > 1u && g.weight_ld * size % 16u)) {
+        return fail(h, LILY_ERR_ARG, "rows of a and weight must start on 16-byte boundaries");
+    }
+    if ((g.tokens > 1u && g.a_ld * size >> 40) || (g.outputs > 1u && g.weight_ld * size >> 40)) {
+        return fail(h, LILY_ERR_CAPACITY, "a row pitch beyond 2^40 bytes");
+    }
+    if (reinterpret_cast<uintptr_t>(g.out) % out_size || reinterpret_cast<uintptr_t>(g.residual) % out_size ||
+        reinterpret_cast<uintptr_t>(g.bias) % (g.bias_dtype == LILY_F32 ? 4u : 2u) ||
+        reinterpret_cast<uintptr_t>(g.a_scales) % 4u || reinterpret_cast<uintptr_t>(g.weight_scales) % 4u) {
+        return fail(h, LILY_ERR_ARG, "a buffer is not aligned to its elements");
+    }
+    if (g.residual == g.out && g.residual_ld != g.out_ld) {
+        return fail(h, LILY_ERR_ARG, "in place means the same pitch");
+    }
+    if (tensor_map_encoder() == nullptr) {
+        return fail(h, LILY_ERR_CUDA, "the driver does not offer cuTensorMapEncodeTiled");
+    }
+    DeviceGuard guard(h->device);
+    LinearArgs a;
+    a.a_scales = g.a_scales, a.w_scales = g.weight_scales;
+    a.bias = g.bias, a.residual = g.residual, a.out = g.out;
+    a.residual_ld = g.residual_ld, a.out_ld = g.out_ld;
+    a.tokens = g.tokens, a.outputs = g.outputs;
+    a.blocks = (uint32_t)(((uint64_t)g.columns * size + BLOCK_BYTES - 1u) / BLOCK_BYTES);
+    a.out_f32 = g.out_dtype == LILY_F32, a.bias_f32 = g.bias_dtype == LILY_F32, a.activation = g.activation;
+    a.status_word = h->status_word, a.wait_ns = h->wait_ns;
+    a.lost_stage = h->lost_stage;
+    h->lost_stage = 0xFFFFFFFFu;  // one launch only
+
+    const uint32_t n = g.tokens <= 16u ? 16u : g.tokens <= 32u ? 32u : g.tokens <= 64u ? 64u : 128u;
+    if (!encode_rows(&a.w_map, g.weight, g.weight_ld, g.outputs, g.columns, g.dtype, TILE_M) ||
+        !encode_rows(&a.a_map, g.a, g.a_ld, g.tokens, g.columns, g.dtype, n)) {
+        return fail(h, LILY_ERR_CUDA, "cuTensorMapEncodeTiled refused a or weight");
+    }
+    a.token_tiles = (g.tokens + n - 1u) / n;
+    const uint64_t tiles = (uint64_t)a.token_tiles * ((g.outputs + TILE_M - 1u) / TILE_M);
+    if (tiles > 0x7FFFFFFFull / 8u) {
+        return fail(h, LILY_ERR_CAPACITY, "more tiles than a launch takes");
+    }
+    // Shares of the columns: as many blocks as the device holds at once, of four steps at least.
+    const uint32_t room = (uint32_t)h->sm_count * (n <= 64u ? 2u : 1u);
+    uint32_t shares = 8u;
+    while (shares > 1u && (tiles * shares > room || a.blocks < 4u * shares)) {
+        shares /= 2u;
+    }
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+    CU(h, e4m3 ? few_by_tokens<true>(a, n, (uint32_t)tiles, shares, stream)
+               : few_by_tokens<false>(a, n, (uint32_t)tiles, shares, stream));
+    return LILY_OK;
+}

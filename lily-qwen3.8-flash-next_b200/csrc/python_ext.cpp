@@ -14,6 +14,7 @@
 #include <cstring>
 #include <vector>
 
+#include "../../include/lily_layers.h"
 #include "../../include/lily_sampler.h"
 
 namespace {
@@ -23,12 +24,14 @@ PyObject *g_names[32];
 enum Name {
     N_UNIFORMS, N_STEPS, N_HISTORY_IDS, N_HISTORY_LEN, N_BIAS_IDS, N_BIAS_VALS, N_BIAS_LEN, N_BAN_IDS, N_BAN_LEN,
     N_FORCED_IDS, N_COUNT_SLOTS, N_OUT_STATUS, N_KEPT_N, N_KEPT_IDS, N_KEPT_PROBS, N_PARAMS_ON_DEVICE, N_MODE, N_Q_DENSE,
-    N_Q_IDS, N_Q_PROBS, N_Q_N, N_U_ACCEPT, N_U_RESID, N_STEP0, N_COUNT_SLOT, N_OUT_LSE, N_COUNT
+    N_Q_IDS, N_Q_PROBS, N_Q_N, N_U_ACCEPT, N_U_RESID, N_STEP0, N_COUNT_SLOT, N_OUT_LSE, N_MASK, N_MASK_ROWS,
+    N_FIRST_ID, N_COUNT
 };
 const char *const kNames[N_COUNT] = {
     "uniforms", "steps", "history_ids", "history_len", "bias_ids", "bias_vals", "bias_len", "ban_ids", "ban_len",
     "forced_ids", "count_slots", "out_status", "kept_n", "kept_ids", "kept_probs", "params_on_device", "mode", "q_dense",
-    "q_ids", "q_probs", "q_n", "u_accept", "u_resid", "step0", "count_slot", "out_lse"};
+    "q_ids", "q_probs", "q_n", "u_accept", "u_resid", "step0", "count_slot", "out_lse", "mask", "mask_rows",
+    "first_id"};
 
 // A call that has to go the other way.
 struct Other {};
@@ -500,6 +503,209 @@ PyObject *py_merge_draw(PyObject *, PyObject *const *v, Py_ssize_t n) {
     });
 }
 
+// The three calls around the head: tensors on the handle's device whose rows are contiguous, of
+// any row pitch. What is not in order goes the other way, which says why.
+struct Rows2 {
+    void *p = nullptr;
+    uint64_t rows = 0, columns = 0, ld = 0;
+    at::ScalarType type = at::kFloat;
+};
+
+Rows2 rows_of(PyObject *o, int device) {
+    Rows2 r;
+    if (o == nullptr || o == Py_None) {
+        return r;
+    }
+    if (!THPVariable_Check(o)) {
+        throw Other();
+    }
+    const at::Tensor &t = THPVariable_Unpack(o);
+    const int64_t dim = t.dim();
+    if (!t.is_cuda() || t.device().index() != device || (dim != 1 && dim != 2) || t.numel() == 0) {
+        throw Other();
+    }
+    r.rows = dim == 2 ? (uint64_t)t.size(0) : 1u;
+    r.columns = (uint64_t)t.size(-1);
+    if ((r.columns > 1u && t.stride(-1) != 1) || (r.rows > 1u && t.stride(0) < (int64_t)r.columns)) {
+        throw Other();
+    }
+    r.ld = r.rows > 1u ? (uint64_t)t.stride(0) : r.columns;
+    r.p = t.data_ptr();
+    r.type = t.scalar_type();
+    return r;
+}
+
+void expect(bool in_order) {
+    if (!in_order) {
+        throw Other();
+    }
+}
+
+// Neighbours in memory: a list of n values.
+template <typename P>
+P *list_of(PyObject *o, int device, uint64_t n, at::ScalarType type) {
+    const Rows2 r = rows_of(o, device);
+    expect(r.p == nullptr || (r.rows * r.columns == n && (r.rows == 1u || r.ld == r.columns) && r.type == type));
+    return static_cast<P *>(r.p);
+}
+
+bool is_word(at::ScalarType t) { return t == at::kInt || t == at::kUInt32; }
+
+template <typename P>
+P *words_at(PyObject *o, int device, uint64_t n) {
+    const Rows2 r = rows_of(o, device);
+    expect(r.p == nullptr || (r.rows * r.columns == n && (r.rows == 1u || r.ld == r.columns) && is_word(r.type)));
+    return static_cast<P *>(r.p);
+}
+
+uint32_t wide_code(at::ScalarType t) {
+    expect(t == at::kFloat || t == at::kBFloat16);
+    return t == at::kFloat ? LILY_F32 : LILY_BF16;
+}
+
+uint32_t any_code(at::ScalarType t) { return t == at::kFloat8_e4m3fn ? (uint32_t)LILY_E4M3 : wide_code(t); }
+
+int device_of(PyObject *o) {
+    expect(PyLong_CheckExact(o));
+    return (int)word(o);
+}
+
+float real(PyObject *o) {
+    expect(PyFloat_CheckExact(o) || PyLong_CheckExact(o));
+    const double d = PyFloat_AsDouble(o);
+    if (d == -1.0 && PyErr_Occurred()) {
+        PyErr_Clear();
+        throw Other();
+    }
+    return (float)d;
+}
+
+// The call's stream: the handle's device's current one for None.
+void *stream_on(PyObject *o, int device) {
+    return o == Py_None ? c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream() : stream_of(o);
+}
+
+// add_rms_norm(handle, device, stream, x, weight, out, residual, residual_out, out_scales, eps, weight_offset)
+PyObject *py_add_rms_norm(PyObject *, PyObject *const *v, Py_ssize_t n) {
+    return guarded(n, 11, [&]() -> int32_t {
+        const int device = device_of(v[1]);
+        const Rows2 x = rows_of(v[3], device), weight = rows_of(v[4], device), out = rows_of(v[5], device),
+                    residual = rows_of(v[6], device), sum = rows_of(v[7], device);
+        expect(x.p && weight.p && out.p && weight.rows == 1u && weight.columns == x.columns);
+        lily_norm_args_t a;
+        std::memset(&a, 0, sizeof a);
+        a.struct_size = sizeof a;
+        expect(x.rows <= 0x7FFFFFFFu && x.columns <= 0x7FFFFFFFu);
+        a.tokens = (uint32_t)x.rows, a.hidden = (uint32_t)x.columns, a.dtype = wide_code(x.type);
+        const auto same = [&](const Rows2 &r) { return r.p == nullptr || (r.rows == x.rows && r.columns == x.columns); };
+        expect(same(out) && same(residual) && same(sum));
+        expect((!residual.p || residual.type == x.type) && (!sum.p || sum.type == x.type));
+        a.x = x.p, a.x_ld = x.ld, a.residual = residual.p, a.residual_ld = residual.ld;
+        a.residual_out = sum.p, a.residual_out_ld = sum.ld;
+        a.weight = weight.p, a.weight_dtype = wide_code(weight.type);
+        a.out = out.p, a.out_ld = out.ld, a.out_dtype = any_code(out.type);
+        a.out_scales = list_of<float>(v[8], device, x.rows, at::kFloat);
+        a.eps = real(v[9]), a.weight_offset = real(v[10]);
+        lily_sampler_t *h = handle(v[0]);
+        void *stream = stream_on(v[2], device);
+        return unlocked([&] { return lily_add_rms_norm(h, stream, &a); });
+    });
+}
+
+// linear(handle, device, stream, a, weight, out, a_scales, weight_scales, bias, activation, residual)
+PyObject *py_linear(PyObject *, PyObject *const *v, Py_ssize_t n) {
+    return guarded(n, 11, [&]() -> int32_t {
+        const int device = device_of(v[1]);
+        const Rows2 x = rows_of(v[3], device), w = rows_of(v[4], device), out = rows_of(v[5], device),
+                    bias = rows_of(v[8], device), residual = rows_of(v[10], device);
+        expect(x.p && w.p && out.p && x.columns == w.columns && out.rows == x.rows && out.columns == w.rows && x.type == w.type);
+        expect(x.rows <= 0x7FFFFFFFu && w.rows <= 0x7FFFFFFFu && x.columns <= 0x7FFFFFFFu);
+        lily_linear_args_t a;
+        std::memset(&a, 0, sizeof a);
+        a.struct_size = sizeof a;
+        a.tokens = (uint32_t)x.rows, a.columns = (uint32_t)x.columns, a.outputs = (uint32_t)w.rows;
+        expect(x.type == at::kBFloat16 || x.type == at::kFloat8_e4m3fn);
+        a.dtype = any_code(x.type), a.out_dtype = wide_code(out.type);
+        a.a = x.p, a.a_ld = x.ld, a.weight = w.p, a.weight_ld = w.ld;
+        a.a_scales = list_of<const float>(v[6], device, x.rows, at::kFloat);
+        a.weight_scales = list_of<const float>(v[7], device, w.rows, at::kFloat);
+        if (bias.p != nullptr) {
+            expect(bias.rows == 1u && bias.columns == w.rows);
+            a.bias = bias.p, a.bias_dtype = wide_code(bias.type);
+        }
+        a.activation = word(v[9]);
+        if (residual.p != nullptr) {
+            expect(residual.rows == out.rows && residual.columns == out.columns && residual.type == out.type);
+            a.residual = residual.p, a.residual_ld = residual.ld;
+        }
+        a.out = out.p, a.out_ld = out.ld;
+        lily_sampler_t *h = handle(v[0]);
+        void *stream = stream_on(v[2], device);
+        return unlocked([&] { return lily_linear(h, stream, &a); });
+    });
+}
+
+// adjust_logits(handle, device, stream, vocab, logits, params, out, keywords)
+PyObject *py_adjust_logits(PyObject *, PyObject *const *v, Py_ssize_t n) {
+    return guarded(n, 8, [&]() -> int32_t {
+        const int device = device_of(v[1]);
+        const Rows2 logits = rows_of(v[4], device), out = rows_of(v[6], device);
+        const uint32_t vocab = word(v[3]);
+        Keywords kw(v[7]);
+        lily_adjust_args_t a;
+        std::memset(&a, 0, sizeof a);
+        a.struct_size = sizeof a;
+        expect(logits.p != nullptr && logits.rows <= 0x7FFFFFFFu && logits.columns == vocab);
+        expect(out.p == nullptr || (out.rows == logits.rows && out.columns == vocab));
+        a.rows = (uint32_t)logits.rows;
+        a.logits = logits.p, a.logits_ld = logits.ld, a.logits_dtype = wide_code(logits.type);
+        const Rows2 &to = out.p != nullptr ? out : logits;
+        a.out = to.p, a.out_ld = to.ld, a.out_dtype = wide_code(to.type);
+        PyObject *on_device = kw.get(N_PARAMS_ON_DEVICE);
+        expect(on_device == nullptr || on_device == Py_False || on_device == Py_True);
+        if (on_device == Py_True) {
+            a.params_on_device = 1;
+            a.params = list_of<const lily_sampling_params_t>(v[5], device, logits.rows * sizeof(lily_sampling_params_t), at::kByte);
+        } else if (v[5] != Py_None) {
+            a.params = params_of(v[5], a.rows);
+        }
+        const auto lists = [&](Name ids, Name len, const uint32_t *&to_ids, const uint32_t *&to_len, uint64_t &ld) -> uint64_t {
+            const Rows2 r = rows_of(kw.get(ids), device);
+            expect(r.p == nullptr || (r.rows == logits.rows && is_word(r.type)));
+            to_ids = static_cast<const uint32_t *>(r.p);
+            to_len = words_at<const uint32_t>(kw.get(len), device, logits.rows);
+            expect((to_ids != nullptr) == (to_len != nullptr));
+            // (What a row's list may hold, not how far rows are apart, bounds its length.)
+            expect(r.rows <= 1u || r.ld == r.columns);
+            ld = r.ld;
+            return r.columns;
+        };
+        lists(N_HISTORY_IDS, N_HISTORY_LEN, a.history_ids, a.history_len, a.history_ld);
+        const uint64_t biases = lists(N_BIAS_IDS, N_BIAS_LEN, a.bias_ids, a.bias_len, a.bias_ld);
+        a.bias_vals = list_of<const float>(kw.get(N_BIAS_VALS), device, logits.rows * biases, at::kFloat);
+        expect((a.bias_vals != nullptr) == (a.bias_ids != nullptr));
+        lists(N_BAN_IDS, N_BAN_LEN, a.ban_ids, a.ban_len, a.ban_ld);
+        if (PyObject *slots = kw.get(N_COUNT_SLOTS)) {
+            a.count_slots = words_of(slots, a.rows, t_rows.slots);
+        }
+        if (PyObject *first = kw.get(N_FIRST_ID)) {
+            a.first_id = word(first);
+            expect(PyLong_AsLongLong(first) == (long long)a.first_id);
+        }
+        const Rows2 mask = rows_of(kw.get(N_MASK), device);
+        if (mask.p != nullptr) {
+            expect(is_word(mask.type) && mask.rows <= 0x7FFFFFFFu && (mask.columns * 32u >= (uint64_t)a.first_id + vocab));
+            a.mask = static_cast<const uint32_t *>(mask.p), a.mask_ld = mask.ld, a.masks = (uint32_t)mask.rows;
+        }
+        a.mask_rows = words_at<const int32_t>(kw.get(N_MASK_ROWS), device, logits.rows);
+        a.out_status = words_at<uint32_t>(kw.get(N_OUT_STATUS), device, logits.rows);
+        kw.done();
+        lily_sampler_t *h = handle(v[0]);
+        void *stream = stream_on(v[2], device);
+        return unlocked([&] { return lily_adjust_logits(h, stream, &a); });
+    });
+}
+
 // bind(SamplingParams)
 PyObject *py_bind(PyObject *, PyObject *type) {
     if (!PyType_Check(type)) {
@@ -525,6 +731,9 @@ PyMethodDef g_methods[] = {{"bind", py_bind, METH_O, nullptr},
                            {"lmhead_logits", fast<py_lmhead_logits>(), METH_FASTCALL, nullptr},
                            {"lmhead_shard_candidates", fast<py_lmhead_shard_candidates>(), METH_FASTCALL, nullptr},
                            {"merge_draw", fast<py_merge_draw>(), METH_FASTCALL, nullptr},
+                           {"add_rms_norm", fast<py_add_rms_norm>(), METH_FASTCALL, nullptr},
+                           {"linear", fast<py_linear>(), METH_FASTCALL, nullptr},
+                           {"adjust_logits", fast<py_adjust_logits>(), METH_FASTCALL, nullptr},
                            {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_lily_calls", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
