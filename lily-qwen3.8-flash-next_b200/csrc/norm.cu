@@ -26,8 +26,35 @@ struct NormArgs {
     void *residual_out, *out;
     float *out_scales;
     uint64_t x_ld, residual_ld, residual_out_ld, out_ld;
-    uint32_t hidden;
+    uint32_t tokens, hidden, weight_f32;
     float inv_hidden, eps, offset;
+};
+
+// How a row's values are dealt out to its threads, eight to a vector.
+enum Deal {
+    ALIGNED,   // rows start on 16-byte boundaries and are a multiple of eight values long: neighbours
+    SHIFTED,   // rows start anywhere, but all tensors' rows alike: neighbours from the boundary before the row's start
+    SCATTERED  // anything else: a block's width apart
+};
+
+// A thread's vector j of a row: the place of its first value (below 0 before a shifted row's start).
+template <Deal D, uint32_t WIDTH>
+struct Vector {
+    int32_t first;
+    uint32_t step;
+    __device__ __forceinline__ Vector(uint32_t j, uint32_t shift) {
+        const uint32_t width = WIDTH ? WIDTH : blockDim.x, t = WIDTH ? threadIdx.x % (WIDTH ? WIDTH : 1u) : threadIdx.x;
+        first = D == SCATTERED ? (int32_t)(j * width * V + t) : (int32_t)((j * width + t) * V) - (int32_t)shift;
+        step = D == SCATTERED ? width : 1u;
+    }
+    // Whether some of its values are the row's; whether all of them are, next to one another.
+    __device__ __forceinline__ bool some(uint32_t n) const { return first < (int32_t)n; }
+    __device__ __forceinline__ bool all(uint32_t n) const {
+        return D == ALIGNED || (D == SHIFTED && first >= 0 && first + (int32_t)V <= (int32_t)n);
+    }
+    __device__ __forceinline__ bool has(uint32_t k, uint32_t n) const {
+        return (uint32_t)(first + (int32_t)(k * step)) < n;
+    }
 };
 
 template <typename T>
@@ -65,28 +92,62 @@ __device__ __forceinline__ void unpack(const Raw<__nv_bfloat16> &r, float (&f)[V
     }
 }
 
-// The V values of a thread's vector j of a row of n: neighbours where the rows allow it (WIDE: they
-// start on 16-byte boundaries and n is a multiple of V), a block's width apart where they do not.
-template <bool WIDE>
-__device__ __forceinline__ uint32_t first_of(uint32_t j) {
-    return WIDE ? (j * blockDim.x + threadIdx.x) * V : j * blockDim.x * V + threadIdx.x;
-}
-
-template <typename T, bool WIDE>
-__device__ __forceinline__ void load(const T *row, uint32_t j, uint32_t n, Raw<T> &r) {
-    const uint32_t i = first_of<WIDE>(j);
-    if (WIDE) {
-        if (i < n) {
-            r = *reinterpret_cast<const Raw<T> *>(row + i);
-        }
-    } else {
+template <typename T, typename Vec>
+__device__ __forceinline__ void load(const T *row, const Vec &v, uint32_t n, Raw<T> &r) {
+    if (v.some(n)) {
+        if (v.all(n)) {
+            r = *reinterpret_cast<const Raw<T> *>(row + v.first);
+        } else {
 #pragma unroll
-        for (uint32_t k = 0; k < V; ++k) {
-            if (i + k * blockDim.x < n) {
-                set(r, k, row[i + k * blockDim.x]);
+            for (uint32_t k = 0; k < V; ++k) {
+                if (v.has(k, n)) {
+                    set(r, k, row[v.first + (int32_t)(k * v.step)]);
+                }
             }
         }
     }
+}
+
+// The weights of a vector, 0 where it has none. `weight` starts on a 16-byte boundary unless the deal is
+// SCATTERED; a shifted vector's lie in two of its vectors.
+template <typename W, Deal D, typename Vec>
+__device__ __forceinline__ void weights(const W *weight, const Vec &v, uint32_t n, uint32_t shift, float (&f)[V]) {
+    Raw<W> r = {};
+    if (D == SHIFTED && shift != 0u && v.all(n) && v.first + (int32_t)shift + (int32_t)V <= (int32_t)n) {
+        float lo[V], hi[V];
+        const W *at = weight + v.first + (int32_t)shift;
+        unpack(*reinterpret_cast<const Raw<W> *>(at - V), lo);
+        unpack(*reinterpret_cast<const Raw<W> *>(at), hi);
+        // f[k] = both[V - shift + k]: by eight, four, two and one, as the shift's bits say.
+        float both[2 * V];
+#pragma unroll
+        for (uint32_t k = 0; k < V; ++k) {
+            both[k] = lo[k];
+            both[V + k] = hi[k];
+        }
+        const uint32_t by = V - shift;
+#pragma unroll
+        for (uint32_t bit = V / 2u; bit > 0u; bit /= 2u) {
+#pragma unroll
+            for (uint32_t k = 0; k + bit < 2u * V; ++k) {
+                both[k] = by & bit ? both[k + bit] : both[k];
+            }
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < V; ++k) {
+            f[k] = both[k];
+        }
+        return;
+    }
+    if (D == SHIFTED && shift != 0u && v.all(n)) {  // (the last whole vector: its second half would end past the weights)
+#pragma unroll
+        for (uint32_t k = 0; k < V; ++k) {
+            set(r, k, weight[v.first + (int32_t)k]);
+        }
+    } else {
+        load<W>(weight, v, n, r);
+    }
+    unpack(r, f);
 }
 
 __device__ __forceinline__ uint32_t two_bf16(float lo, float hi) {
@@ -120,54 +181,65 @@ __device__ __forceinline__ void put_one(__nv_fp8_e4m3 *to, float f) {
     to->__x = __nv_cvt_float_to_fp8(f, __NV_SATFINITE, __NV_E4M3);
 }
 
-template <typename T, bool WIDE>
-__device__ __forceinline__ void store(T *row, uint32_t j, uint32_t n, const float (&f)[V]) {
-    const uint32_t i = first_of<WIDE>(j);
-    if (WIDE) {
-        if (i < n) {
-            put(row + i, f);
-        }
-    } else {
+template <typename T, typename Vec>
+__device__ __forceinline__ void store(T *row, const Vec &v, uint32_t n, const float (&f)[V]) {
+    if (v.some(n)) {
+        if (v.all(n)) {
+            put(row + v.first, f);
+        } else {
 #pragma unroll
-        for (uint32_t k = 0; k < V; ++k) {
-            if (i + k * blockDim.x < n) {
-                put_one(row + i + k * blockDim.x, f[k]);
+            for (uint32_t k = 0; k < V; ++k) {
+                if (v.has(k, n)) {
+                    put_one(row + v.first + (int32_t)(k * v.step), f[k]);
+                }
             }
         }
     }
 }
 
-// T: x's type, W: the weight's, O: out's; VECS vectors a thread. Values past a row's end are 0
-// in registers.
-template <typename T, typename W, typename O, uint32_t VECS, bool WIDE>
-__global__ void __launch_bounds__(1024) add_rms_norm_kernel(const __grid_constant__ NormArgs a) {
+// T: x's type, O: out's; VECS vectors a thread. WARPS 0: a block per token; else a warp per token,
+// WARPS of them in a block. Values past a row's ends are 0 in registers.
+template <typename T, typename O, uint32_t VECS, Deal D, uint32_t WARPS>
+__global__ void __launch_bounds__(WARPS ? 32u * WARPS : VECS == 1u ? 1024u : 512u) add_rms_norm_kernel(const __grid_constant__ NormArgs a) {
     __shared__ float part_sum[32];
     __shared__ uint32_t part_max[32];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     constexpr bool CODES = sizeof(O) == 1;
+    using Vec = Vector<D, WARPS ? 32u : 0u>;
     const uint32_t t = threadIdx.x, n = a.hidden;
-    const uint64_t token = blockIdx.x;
-    // All of it is asked for before any of it is used, as far as 64 registers hold it.
-    constexpr bool EARLY_RESIDUAL = VECS * sizeof(T) <= 8, EARLY_WEIGHT = VECS * (2 * sizeof(T) + sizeof(W)) <= 12;
-    Raw<T> x[VECS] = {}, residual[EARLY_RESIDUAL ? VECS : 1] = {};
-    Raw<W> weight[EARLY_WEIGHT ? VECS : 1] = {};
+    const uint64_t token = WARPS ? blockIdx.x * WARPS + t / 32u : blockIdx.x;
+    if (WARPS && token >= a.tokens) {
+        return;
+    }
     const T *x_row = static_cast<const T *>(a.x) + token * a.x_ld;
+    const uint32_t shift = D == SHIFTED ? (uint32_t)(reinterpret_cast<uintptr_t>(x_row) / sizeof(T)) % V : 0u;
+    // All of it is asked for before any of it is used, as far as the registers hold it.
+    constexpr bool EARLY = VECS * sizeof(T) <= 8;
+    Raw<T> x[VECS] = {}, residual[EARLY ? VECS : 1] = {};
 #pragma unroll
     for (uint32_t j = 0; j < VECS; ++j) {
-        load<T, WIDE>(x_row, j, n, x[j]);
+        load<T>(x_row, Vec(j, shift), n, x[j]);
     }
     const T *residual_row = static_cast<const T *>(a.residual) + token * a.residual_ld;
-    if (EARLY_RESIDUAL && a.residual != nullptr) {
+    if (EARLY && a.residual != nullptr) {
 #pragma unroll
         for (uint32_t j = 0; j < VECS; ++j) {
-            load<T, WIDE>(residual_row, j, n, residual[j]);
+            load<T>(residual_row, Vec(j, shift), n, residual[j]);
         }
     }
-    if (EARLY_WEIGHT) {
+    float w[EARLY ? VECS : 1][V];
+    const auto weights_of = [&](uint32_t j, float (&f)[V]) {
+        if (a.weight_f32) {
+            weights<float, D>(static_cast<const float *>(a.weight), Vec(j, shift), n, shift, f);
+        } else {
+            weights<__nv_bfloat16, D>(static_cast<const __nv_bfloat16 *>(a.weight), Vec(j, shift), n, shift, f);
+        }
+    };
+    if (EARLY) {
 #pragma unroll
         for (uint32_t j = 0; j < VECS; ++j) {
-            load<W, WIDE>(static_cast<const W *>(a.weight), j, n, weight[j]);
+            weights_of(j, w[j]);
         }
     }
     T *residual_out = static_cast<T *>(a.residual_out) + token * a.residual_out_ld;
@@ -176,29 +248,28 @@ __global__ void __launch_bounds__(1024) add_rms_norm_kernel(const __grid_constan
     uint32_t largest = 0u;
 #pragma unroll
     for (uint32_t j = 0; j < VECS; ++j) {
-        float f[V];
         unpack(x[j], u[j]);
         if (a.residual != nullptr) {
-            if (!EARLY_RESIDUAL) {
-                load<T, WIDE>(residual_row, j, n, residual[0] = {});
+            float f[V];
+            if (!EARLY) {
+                load<T>(residual_row, Vec(j, shift), n, residual[0] = {});
             }
-            unpack(residual[EARLY_RESIDUAL ? j : 0], f);
+            unpack(residual[EARLY ? j : 0], f);
 #pragma unroll
             for (uint32_t k = 0; k < V; ++k) {
                 u[j][k] += f[k];
             }
         }
         if (a.residual_out != nullptr) {
-            store<T, WIDE>(residual_out, j, n, u[j]);
+            store<T>(residual_out, Vec(j, shift), n, u[j]);
         }
-        if (!EARLY_WEIGHT) {
-            load<W, WIDE>(static_cast<const W *>(a.weight), j, n, weight[0] = {});
+        if (!EARLY) {
+            weights_of(j, w[0]);
         }
-        unpack(weight[EARLY_WEIGHT ? j : 0], f);
 #pragma unroll
         for (uint32_t k = 0; k < V; ++k) {
             sum = fmaf(u[j][k], u[j][k], sum);
-            u[j][k] *= a.offset + f[k];
+            u[j][k] *= a.offset + w[EARLY ? j : 0][k];
             if (CODES) {
                 largest = max(largest, __float_as_uint(u[j][k]) & 0x7FFFFFFFu);
             }
@@ -212,22 +283,26 @@ __global__ void __launch_bounds__(1024) add_rms_norm_kernel(const __grid_constan
         largest = __reduce_max_sync(0xFFFFFFFFu, largest);
     }
     const uint32_t warps = blockDim.x / 32u, lane = t % 32u;
-    if (lane == 0u) {
-        part_sum[t / 32u] = sum;
-        part_max[t / 32u] = largest;
-    }
-    __syncthreads();
-    sum = lane < warps ? part_sum[lane] : 0.0f;
+    if (WARPS == 0u) {
+        if (lane == 0u) {
+            part_sum[t / 32u] = sum;
+            part_max[t / 32u] = largest;
+        }
+        __syncthreads();
+        sum = lane < warps ? part_sum[lane] : 0.0f;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+        for (int o = 16; o > 0; o >>= 1) {
+            sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+        }
+        if (CODES) {
+            largest = __reduce_max_sync(0xFFFFFFFFu, lane < warps ? part_max[lane] : 0u);
+        }
     }
     float factor = 1.0f / sqrtf(fmaf(sum, a.inv_hidden, a.eps));
     if (CODES) {
-        largest = __reduce_max_sync(0xFFFFFFFFu, lane < warps ? part_max[lane] : 0u);
         float m = __uint_as_float(largest) * factor;
         m = m < 0x1p-64f ? 0x1p-64f : m;  // (a NaN stays)
-        if (t == 0u) {
+        if (WARPS ? lane == 0u : t == 0u) {
             a.out_scales[token] = m / E4M3_MAX;
         }
         factor *= E4M3_MAX / m;
@@ -239,56 +314,61 @@ __global__ void __launch_bounds__(1024) add_rms_norm_kernel(const __grid_constan
         for (uint32_t k = 0; k < V; ++k) {
             u[j][k] *= factor;
         }
-        store<O, WIDE>(out, j, n, u[j]);
+        store<O>(out, Vec(j, shift), n, u[j]);
     }
 }
 
-template <typename T, typename W, typename O, uint32_t VECS, bool WIDE>
-cudaError_t launch_norm(const NormArgs &a, uint32_t tokens, cudaStream_t stream) {
-    const uint32_t per = V * VECS;
+template <typename T, typename O, uint32_t VECS, Deal D, uint32_t WARPS>
+cudaError_t launch_norm(const NormArgs &a, cudaStream_t stream) {
+    const uint32_t per = V * VECS, values = a.hidden + (D == SHIFTED ? V - 1u : 0u);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(tokens, 1, 1);
-    cfg.blockDim = dim3((((a.hidden + per - 1u) / per) + 31u) & ~31u, 1, 1);
+    cfg.gridDim = dim3(WARPS ? (a.tokens + WARPS - 1u) / (WARPS ? WARPS : 1u) : a.tokens, 1, 1);
+    cfg.blockDim = dim3(WARPS ? 32u * WARPS : (((values + per - 1u) / per) + 31u) & ~31u, 1, 1);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, add_rms_norm_kernel<T, W, O, VECS, WIDE>, a);
+    return cudaLaunchKernelEx(&cfg, add_rms_norm_kernel<T, O, VECS, D, WARPS>, a);
 }
 
-#ifndef NORM_FEW
-#define NORM_FEW 296
-#endif
-#ifndef NORM_MANY
-#define NORM_MANY 2u
-#endif
-template <typename T, typename W, typename O>
-cudaError_t norm_by_size(const NormArgs &a, uint32_t tokens, bool wide, cudaStream_t stream) {
-    const uint32_t least = a.hidden > 16384u ? 4u : a.hidden > 8192u ? 2u : 1u;
-    const uint32_t vecs = std::max(least, tokens > NORM_FEW ? NORM_MANY : 1u);
-    if (vecs == 4u) {
-        return wide ? launch_norm<T, W, O, 4, true>(a, tokens, stream) : launch_norm<T, W, O, 4, false>(a, tokens, stream);
+template <typename T, typename O>
+cudaError_t norm_by_size(const NormArgs &a, Deal deal, bool many, cudaStream_t stream) {
+    constexpr uint32_t WARPS = 8;
+    if (deal == SCATTERED) {
+        return a.hidden <= 8192u ? launch_norm<T, O, 1, SCATTERED, 0>(a, stream) : launch_norm<T, O, 8, SCATTERED, 0>(a, stream);
     }
-    if (vecs == 2u) {
-        return wide ? launch_norm<T, W, O, 2, true>(a, tokens, stream) : launch_norm<T, W, O, 2, false>(a, tokens, stream);
+    // Many short rows: a warp each, with nothing to wait for (16384 x 512 bf16 to codes 17.5 -> 10.4 us, floor 9.0).
+    if (many && deal == ALIGNED && a.hidden <= 1024u) {
+        return a.hidden <= 256u   ? launch_norm<T, O, 1, ALIGNED, WARPS>(a, stream)
+               : a.hidden <= 512u ? launch_norm<T, O, 2, ALIGNED, WARPS>(a, stream)
+                                  : launch_norm<T, O, 4, ALIGNED, WARPS>(a, stream);
     }
-    return wide ? launch_norm<T, W, O, 1, true>(a, tokens, stream) : launch_norm<T, W, O, 1, false>(a, tokens, stream);
-}
-
-template <typename T, typename W>
-cudaError_t norm_by_out(const NormArgs &a, uint32_t out_dtype, uint32_t tokens, bool wide, cudaStream_t stream) {
-    return out_dtype == LILY_F32    ? norm_by_size<T, W, float>(a, tokens, wide, stream)
-           : out_dtype == LILY_BF16 ? norm_by_size<T, W, __nv_bfloat16>(a, tokens, wide, stream)
-                                    : norm_by_size<T, W, __nv_fp8_e4m3>(a, tokens, wide, stream);
+    // Few tokens (two blocks an SM or less): as many threads as there are vectors, the shortest way
+    // through a block. Many: blocks of 256 threads or so, whose loads in flight come from several vectors a thread:
+    // 16384 x 4096 bf16 to codes 77.3 us with one vector a thread, 72.0 with two and 72.5 with four (floor
+    // 71.8); 8000 x 8192 f32 to codes 69.4, 66.2 and 51.7 (50.1). A row that misses the boundaries costs a
+    // tenth more than one that does not (777 x 5001 and 5008 f32: 9.8 and 9.0 us, scattered 15.7).
+    const uint32_t vectors = (a.hidden + (deal == SHIFTED ? 2u * V - 2u : V - 1u)) / V, threads = many ? 256u : 1024u;
+    const uint32_t vecs = vectors > 2048u ? 8u : vectors > std::min(1024u, 2u * threads) ? 4u : vectors > threads ? 2u : 1u;
+    if (deal == ALIGNED) {
+        return vecs == 8u   ? launch_norm<T, O, 8, ALIGNED, 0>(a, stream)
+               : vecs == 4u ? launch_norm<T, O, 4, ALIGNED, 0>(a, stream)
+               : vecs == 2u ? launch_norm<T, O, 2, ALIGNED, 0>(a, stream)
+                            : launch_norm<T, O, 1, ALIGNED, 0>(a, stream);
+    }
+    return vecs == 8u   ? launch_norm<T, O, 8, SHIFTED, 0>(a, stream)
+           : vecs == 4u ? launch_norm<T, O, 4, SHIFTED, 0>(a, stream)
+           : vecs == 2u ? launch_norm<T, O, 2, SHIFTED, 0>(a, stream)
+                        : launch_norm<T, O, 1, SHIFTED, 0>(a, stream);
 }
 
 template <typename T>
-cudaError_t norm_by_weight(const NormArgs &a, uint32_t weight_dtype, uint32_t out_dtype, uint32_t tokens, bool wide,
-                           cudaStream_t stream) {
-    return weight_dtype == LILY_F32 ? norm_by_out<T, float>(a, out_dtype, tokens, wide, stream)
-                                    : norm_by_out<T, __nv_bfloat16>(a, out_dtype, tokens, wide, stream);
+cudaError_t norm_by_out(const NormArgs &a, uint32_t out_dtype, Deal deal, bool many, cudaStream_t stream) {
+    return out_dtype == LILY_F32    ? norm_by_size<T, float>(a, deal, many, stream)
+           : out_dtype == LILY_BF16 ? norm_by_size<T, __nv_bfloat16>(a, deal, many, stream)
+                                    : norm_by_size<T, __nv_fp8_e4m3>(a, deal, many, stream);
 }
 
 uint32_t element(uint32_t dtype) { return dtype == LILY_F32 ? 4u : dtype == LILY_BF16 ? 2u : 1u; }
@@ -354,13 +434,26 @@ extern "C" int32_t lily_add_rms_norm(lily_sampler_t *h, void *stream, const lily
     a.hidden = g.hidden;
     a.inv_hidden = 1.0f / (float)g.hidden;
     a.eps = g.eps, a.offset = g.weight_offset;
-    const bool wide = g.hidden % V == 0u && rows_at(g.x, g.x_ld, g.dtype, g.tokens, 16u) &&
-                      rows_at(g.residual, g.residual_ld, g.dtype, g.tokens, 16u) &&
-                      rows_at(g.residual_out, g.residual_out_ld, g.dtype, g.tokens, 16u) &&
-                      rows_at(g.out, g.out_ld, g.out_dtype, g.tokens, g.out_dtype == LILY_E4M3 ? 8u : 16u) &&
-                      reinterpret_cast<uintptr_t>(g.weight) % 16u == 0u;
+    a.tokens = g.tokens, a.weight_f32 = g.weight_dtype == LILY_F32;
+    // The deal: rows 16 bytes at a time where they allow it, or where all of them miss a boundary of
+    // eight values alike.
+    Deal deal = SCATTERED;
+    if (reinterpret_cast<uintptr_t>(g.weight) % 16u == 0u) {
+        const auto miss = [&](const void *p, uint32_t dtype) { return (uint32_t)(reinterpret_cast<uintptr_t>(p) / element(dtype) % V); };
+        const auto alike = [&](const void *p, uint64_t ld, uint32_t dtype) {
+            return p == nullptr || (miss(p, dtype) == miss(g.x, g.dtype) && (g.tokens == 1u || ld % V == g.x_ld % V));
+        };
+        if (alike(g.residual, g.residual_ld, g.dtype) && alike(g.residual_out, g.residual_out_ld, g.dtype) &&
+            alike(g.out, g.out_ld, g.out_dtype)) {
+            deal = g.hidden % V == 0u && miss(g.x, g.dtype) == 0u && (g.tokens == 1u || g.x_ld % V == 0u) ? ALIGNED : SHIFTED;
+        }
+    }
+    if (deal == SHIFTED && g.hidden > LILY_NORM_MAX_HIDDEN - V) {
+        deal = SCATTERED;  // (a shifted row takes one vector more than the largest block's threads have)
+    }
+    const bool many = g.tokens > 2u * (uint32_t)h->sm_count;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    CU(h, g.dtype == LILY_F32 ? norm_by_weight<float>(a, g.weight_dtype, g.out_dtype, g.tokens, wide, s)
-                              : norm_by_weight<__nv_bfloat16>(a, g.weight_dtype, g.out_dtype, g.tokens, wide, s));
+    CU(h, g.dtype == LILY_F32 ? norm_by_out<float>(a, g.out_dtype, deal, many, s)
+                              : norm_by_out<__nv_bfloat16>(a, g.out_dtype, deal, many, s));
     return LILY_OK;
 }
