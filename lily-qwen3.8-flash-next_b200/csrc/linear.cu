@@ -43,18 +43,32 @@ struct LinearArgs {
     uint32_t lost_stage;    // test hook: the first block leaves out the copies of this step (~0: none)
 };
 
-__device__ __forceinline__ float activated(float v, uint32_t activation) {
-    switch (activation) {
-        case LILY_ACT_RELU:
-            return v < 0.0f ? 0.0f : v;  // (a NaN stays)
-        case LILY_ACT_SILU:
-            return v / (1.0f + expf(-v));
-        case LILY_ACT_GELU:
-            return 0.5f * v * (1.0f + erff(v * 0.70710678f));
-        case LILY_ACT_GELU_TANH:
-            return 0.5f * v * (1.0f + tanhf(0.79788456f * (v + 0.044715f * v * v * v)));
-        default:
-            return v;
+// Sixteen values through the activation. One branch for all of them: with the branch inside, sixteen
+// copies of every function's code lay in the epilogue's loop, which then ran from instruction misses
+// (4099 x 4096 x 4096 without an activation 120 us, with a residual 331).
+__device__ __forceinline__ void activate(float (&v)[16], uint32_t activation) {
+    if (activation == LILY_ACT_NONE) {
+    } else if (activation == LILY_ACT_RELU) {
+#pragma unroll
+        for (uint32_t j = 0; j < 16u; ++j) {
+            v[j] = v[j] < 0.0f ? 0.0f : v[j];  // (a NaN stays)
+        }
+    } else if (activation == LILY_ACT_SILU) {
+#pragma unroll
+        for (uint32_t j = 0; j < 16u; ++j) {
+            v[j] = __fdividef(v[j], 1.0f + expf(-v[j]));
+        }
+    } else if (activation == LILY_ACT_GELU) {
+#pragma unroll
+        for (uint32_t j = 0; j < 16u; ++j) {
+            v[j] = 0.5f * v[j] * (1.0f + erff(v[j] * 0.70710678f));
+        }
+    } else {
+#pragma unroll
+        for (uint32_t j = 0; j < 16u; ++j) {
+            const float u = 0.79788456f * (v[j] + 0.044715f * v[j] * v[j] * v[j]);
+            v[j] = __fdividef(v[j], 1.0f + expf(-2.0f * u));  // (1 + tanh(u)) / 2 = 1 / (1 + exp(-2 u))
+        }
     }
 }
 
@@ -76,21 +90,67 @@ __device__ __forceinline__ Output output_of(const LinearArgs &a, uint32_t n) {
     return o;
 }
 
-__device__ __forceinline__ float residual_at(const LinearArgs &a, uint32_t t, uint32_t n) {
-    const uint64_t at = (uint64_t)t * a.residual_ld + n;
-    return a.out_f32 ? static_cast<const float *>(a.residual)[at]
-                     : __bfloat162float(static_cast<const __nv_bfloat16 *>(a.residual)[at]);
+// The residuals of output n and of up to sixteen tokens from t on.
+__device__ __forceinline__ void residuals_of(const LinearArgs &a, const Output &o, uint32_t t, uint32_t n, uint32_t live,
+                                             float (&r)[16]) {
+    if (a.residual == nullptr || !o.live) {
+#pragma unroll
+        for (uint32_t j = 0; j < 16u; ++j) {
+            r[j] = 0.0f;
+        }
+    } else if (a.out_f32) {
+        const float *p = static_cast<const float *>(a.residual) + (uint64_t)t * a.residual_ld + n;
+#pragma unroll
+        for (uint32_t j = 0; j < 16u; ++j) {
+            r[j] = j < live ? p[j * a.residual_ld] : 0.0f;
+        }
+    } else {
+        const __nv_bfloat16 *p = static_cast<const __nv_bfloat16 *>(a.residual) + (uint64_t)t * a.residual_ld + n;
+#pragma unroll
+        for (uint32_t j = 0; j < 16u; ++j) {
+            r[j] = j < live ? __bfloat162float(p[j * a.residual_ld]) : 0.0f;
+        }
+    }
 }
 
-__device__ __forceinline__ void finish(const LinearArgs &a, const Output &o, uint32_t t, uint32_t n, float sum,
-                                       float residual) {
-    float v = a.a_scales != nullptr ? sum * (__ldg(a.a_scales + t) * o.scale) : sum;
-    v = activated(v + o.bias, a.activation) + residual;
-    const uint64_t at = (uint64_t)t * a.out_ld + n;
-    if (a.out_f32) {
-        static_cast<float *>(a.out)[at] = v;
+// The sums v of output n and of up to sixteen tokens from t on, finished and written. (A whole warp:
+// lane j has token j's scale.)
+__device__ __forceinline__ void finish(const LinearArgs &a, const Output &o, uint32_t t, uint32_t n, uint32_t live, float (&v)[16],
+                                       const float (&r)[16]) {
+    if (a.a_scales != nullptr) {
+        const uint32_t lane = threadIdx.x % 32u;
+        const float mine = lane < min(live, 16u) ? __ldg(a.a_scales + t + lane) : 0.0f;
+#pragma unroll
+        for (uint32_t j = 0; j < 16u; ++j) {
+            v[j] *= __shfl_sync(FULL, mine, j) * o.scale;
+        }
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < 16u; ++j) {
+        v[j] += o.bias;
+    }
+    activate(v, a.activation);
+#pragma unroll
+    for (uint32_t j = 0; j < 16u; ++j) {
+        v[j] += r[j];
+    }
+    if (!o.live) {
+    } else if (a.out_f32) {
+        float *p = static_cast<float *>(a.out) + (uint64_t)t * a.out_ld + n;
+#pragma unroll
+        for (uint32_t j = 0; j < 16u; ++j) {
+            if (j < live) {
+                p[j * a.out_ld] = v[j];
+            }
+        }
     } else {
-        static_cast<__nv_bfloat16 *>(a.out)[at] = __float2bfloat16_rn(v);
+        __nv_bfloat16 *p = static_cast<__nv_bfloat16 *>(a.out) + (uint64_t)t * a.out_ld + n;
+#pragma unroll
+        for (uint32_t j = 0; j < 16u; ++j) {
+            if (j < live) {
+                p[j * a.out_ld] = __float2bfloat16_rn(v[j]);
+            }
+        }
     }
 }
 
@@ -277,17 +337,9 @@ __global__ void __launch_bounds__(192) linear_few_kernel(const __grid_constant__
             tc_fence_after();
             for (uint32_t c = 0; c < live; c += 16u) {
                 float v[16], r[16];
-#pragma unroll
-                for (uint32_t j = 0; j < 16u; ++j) {
-                    r[j] = a.residual != nullptr && o.live && c + j < live ? residual_at(a, token0 + c + j, n) : 0.0f;
-                }
+                residuals_of(a, o, token0 + c, n, live - c, r);
                 sums_of(c, v);
-#pragma unroll
-                for (uint32_t j = 0; j < 16u; ++j) {
-                    if (o.live && c + j < live) {
-                        finish(a, o, token0 + c + j, n, v[j], r[j]);
-                    }
-                }
+                finish(a, o, token0 + c, n, live - c, v, r);
             }
         }
     } else {
@@ -317,15 +369,20 @@ __global__ void __launch_bounds__(192) linear_few_kernel(const __grid_constant__
         if (warp >= 2u) {
             const Output o = output_of(a, n);
             const float *part = reinterpret_cast<const float *>(smem + S::PART) + row;
-            for (uint32_t c = rank * per; c < min(live, (rank + 1u) * per); ++c) {
-                const float r = a.residual != nullptr && o.live ? residual_at(a, token0 + c, n) : 0.0f;
-                float v = part[c % per * TILE_M];
-                for (uint32_t k = 1; k < shares; ++k) {
-                    v += part[(k * per + c % per) * TILE_M];
+            const uint32_t first = rank * per, mine = first < live ? min(per, live - first) : 0u;
+            for (uint32_t c = 0; c < mine; c += 16u) {
+                float v[16], r[16];
+                residuals_of(a, o, token0 + first + c, n, mine - c, r);
+#pragma unroll
+                for (uint32_t j = 0; j < 16u; ++j) {
+                    v[j] = 0.0f;
+                    if (c + j < mine) {
+                        for (uint32_t k = 0; k < shares; ++k) {
+                            v[j] += part[(k * per + c + j) * TILE_M];
+                        }
+                    }
                 }
-                if (o.live) {
-                    finish(a, o, token0 + c, n, v, r);
-                }
+                finish(a, o, token0 + first + c, n, mine - c, v, r);
             }
         }
     }
@@ -335,6 +392,243 @@ __global__ void __launch_bounds__(192) linear_few_kernel(const __grid_constant__
     tc_fence_after();
     if (warp == 1u) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::COLS) : "memory");
+    }
+    if (tid == 0 && *abort_word) {
+        atomicOr(a.status_word, 1u << lily_head::STATUS_TIMEOUT_BIT);
+    }
+}
+
+// ----------------------------------------------------------------- many tokens --
+//
+// Tiles of 256 outputs x 256 tokens, each by a pair of blocks (a cluster of two on neighbouring
+// SMs) whose tensor cores multiply together: either block holds 128 outputs' weights and 128 tokens in
+// shared memory, and the pair's multiply reads both. That halves the bytes that a multiply takes
+// out of each SM's shared memory, which one block alone is bound by. The pairs stay for all of the launch; an
+// accumulator is finished (scale, bias, activation, residual) while the next tile is multiplied
+// into the other one.
+//
+// A block's warps: 0 asks for the block's copies, 1 issues the pair's multiplies (in the first block
+// of the pair alone), 2 to 9 are the epilogue, two for each quarter of tensor memory's lanes.
+struct Many {
+    static constexpr uint32_t THREADS = 320;
+    static constexpr uint32_t TILE = 256;          // of outputs and of tokens
+    static constexpr uint32_t STAGES = 6;
+    static constexpr uint32_t STAGE = 2u * A_STAGE;  // a block's half of the weights, and of the tokens
+    static constexpr uint32_t ACCS = 2;
+    static constexpr uint32_t EPI_WARPS = 8;
+    static constexpr uint32_t COLS = ACCS * TILE;
+    static constexpr uint32_t FULL_BARS = STAGES * STAGE;           // in the first block: both blocks' copies are there
+    static constexpr uint32_t EMPTY = FULL_BARS + 8u * STAGES;
+    static constexpr uint32_t ACC_FULL = EMPTY + 8u * STAGES;
+    static constexpr uint32_t ACC_EMPTY = ACC_FULL + 8u * ACCS;     // in the first block: both blocks have read it
+    static constexpr uint32_t FINAL = ACC_EMPTY + 8u * ACCS;
+    static constexpr uint32_t TMEM_ADDR = FINAL + 8u;
+    static constexpr uint32_t ABORT = TMEM_ADDR + 4u;
+    static constexpr uint32_t BYTES = ABORT + 4u + 1024u;
+    static_assert(BYTES <= 227u * 1024u, "shared memory of one block");
+};
+
+__device__ __forceinline__ uint32_t at_rank(uint32_t addr, uint32_t rank) {
+    uint32_t there;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(addr), "r"(rank));
+    return there;
+}
+
+// A copy into this block's shared memory whose bytes complete a barrier of either block of the pair.
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap *map, uint32_t cluster_bar, int32_t x, int32_t y) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(cluster_bar), "r"(x), "r"(y)
+        : "memory");
+}
+
+template <bool E4M3>
+__device__ __forceinline__ void mma_ss_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    if (E4M3) {
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+            ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+            : "memory");
+    } else {
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+            ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+            : "memory");
+    }
+}
+
+// Arrives at this barrier of both blocks once the multiplies issued so far have run.
+__device__ __forceinline__ void mma_commit_pair(uint32_t bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+        "h"((uint16_t)3)
+        : "memory");
+}
+
+template <bool E4M3>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(320, 1) linear_many_kernel(const __grid_constant__ LinearArgs a) {
+    using S = Many;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t *smem = smem_raw + (base - smem_u32(smem_raw));
+    volatile uint32_t *abort_word = reinterpret_cast<volatile uint32_t *>(smem + S::ABORT);
+    const uint32_t tid = threadIdx.x, warp = __shfl_sync(FULL, tid / 32u, 0), lane = tid % 32u;
+    uint32_t rank;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    const uint32_t pair = blockIdx.x / 2u, pairs = gridDim.x / 2u;
+    const uint32_t output_tiles = (a.outputs + S::TILE - 1u) / S::TILE, tiles = output_tiles * a.token_tiles;
+
+    if (tid == 0) {
+        for (uint32_t s = 0; s < S::STAGES; ++s) {
+            mbar_init(base + S::FULL_BARS + 8 * s, 1);
+            mbar_init(base + S::EMPTY + 8 * s, 1);
+        }
+        for (uint32_t b = 0; b < S::ACCS; ++b) {
+            mbar_init(base + S::ACC_FULL + 8 * b, 1);
+            mbar_init(base + S::ACC_EMPTY + 8 * b, 2u * S::EPI_WARPS);
+        }
+        mbar_init(base + S::FINAL, 1);
+        *abort_word = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1u) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + S::TMEM_ADDR),
+                     "r"(S::COLS)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_arrive();
+    cluster_wait();  // (both blocks' barriers and tensor memory are there)
+    tc_fence_after();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(smem + S::TMEM_ADDR);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (behind the allocation, as above)
+
+    if (warp == 0u) {
+        if (lane == 0u) {
+            uint32_t i = 0;  // steps so far
+            bool gave_up = false;
+            for (uint32_t tile = pair; tile < tiles && !gave_up; tile += pairs) {
+                const int32_t output0 = (int32_t)(tile / a.token_tiles * S::TILE + rank * TILE_M);
+                const int32_t token0 = (int32_t)(tile % a.token_tiles * S::TILE + rank * TILE_M);
+                for (uint32_t k = 0; k < a.blocks; ++k, ++i) {
+                    const uint32_t s = i % S::STAGES;
+                    if (mbar_wait(base + S::EMPTY + 8 * s, (i / S::STAGES & 1u) ^ 1u, abort_word, a.wait_ns)) {
+                        gave_up = true;
+                        break;
+                    }
+                    const uint32_t bar = base + S::FULL_BARS + 8 * s, to = base + s * S::STAGE;
+                    const int32_t x = (int32_t)(k * (E4M3 ? BLOCK_BYTES : BLOCK_BYTES / 2u));
+                    if (i == a.lost_stage && pair == 0u && rank == 0u) {
+                        continue;  // (test hook: the stage never fills)
+                    }
+                    if (rank == 0u) {
+                        mbar_expect_tx(bar, 2u * S::STAGE);
+                    }
+                    tma_load_2d_pair(to, &a.w_map, at_rank(bar, 0), x, output0);
+                    tma_load_2d_pair(to + A_STAGE, &a.a_map, at_rank(bar, 0), x, token0);
+                }
+            }
+            if (gave_up) {
+                // The copies asked for land in this block's shared memory, but are counted at the
+                // first block's barriers: this one stays for a millisecond, which no copy takes.
+                for (const uint64_t t0 = global_ns(); global_ns() - t0 < 1000000u;) {
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1u && rank == 0u) {
+        const bool leader = elect_one();
+        const uint32_t idesc = product_desc<E4M3>(2u * TILE_M, S::TILE);
+        uint32_t i = 0, turn = 0;
+        bool gave_up = false;
+        for (uint32_t tile = pair; tile < tiles && !gave_up; tile += pairs, ++turn) {
+            const uint32_t b = turn % S::ACCS;
+            if (warp_wait(base + S::ACC_EMPTY + 8 * b, (turn / S::ACCS & 1u) ^ 1u, abort_word, a.wait_ns)) {
+                break;
+            }
+            for (uint32_t k = 0; k < a.blocks; ++k, ++i) {
+                const uint32_t s = i % S::STAGES;
+                if (warp_wait(base + S::FULL_BARS + 8 * s, i / S::STAGES & 1u, abort_word, a.wait_ns)) {
+                    gave_up = true;
+                    break;
+                }
+                tc_fence_after();
+                if (leader) {
+                    const uint64_t adesc = operand_desc(base + s * S::STAGE), bdesc = operand_desc(base + s * S::STAGE + A_STAGE);
+#pragma unroll
+                    for (uint32_t q = 0; q < 4u; ++q) {
+                        mma_ss_pair<E4M3>(tmem + b * S::TILE, adesc + 2u * q, bdesc + 2u * q, idesc, k > 0u || q > 0u);
+                    }
+                    mma_commit_pair(base + S::EMPTY + 8 * s);
+                }
+                __syncwarp();
+            }
+            if (leader && !gave_up) {
+                mma_commit_pair(base + S::ACC_FULL + 8 * b);
+            }
+            __syncwarp();
+        }
+        if (leader) {
+            mma_commit_pair(base + S::FINAL);
+            mbar_drain(base + S::FINAL, 0u, a.wait_ns);  // (nothing is freed under a multiply, on any way out)
+        }
+        __syncwarp();
+    } else if (warp >= 2u) {
+        const uint32_t quad = warp % 4u, half = (warp - 2u) / 4u;
+        uint32_t turn = 0;
+        for (uint32_t tile = pair; tile < tiles; tile += pairs, ++turn) {
+            const uint32_t b = turn % S::ACCS;
+            const uint32_t n = tile / a.token_tiles * S::TILE + rank * TILE_M + quad * 32u + lane;
+            const uint32_t token0 = tile % a.token_tiles * S::TILE + half * (S::TILE / 2u);
+            const uint32_t live = token0 < a.tokens ? min(S::TILE / 2u, a.tokens - token0) : 0u;
+            const uint32_t from = tmem + (quad * 32u << 16) + b * S::TILE + half * (S::TILE / 2u);
+            const Output o = output_of(a, n);
+            float r[16];
+            residuals_of(a, o, token0, n, live, r);
+            if (warp_wait(base + S::ACC_FULL + 8 * b, turn / S::ACCS & 1u, abort_word, a.wait_ns)) {
+                break;
+            }
+            tc_fence_after();
+            for (uint32_t c = 0; c < live; c += 16u) {
+                uint32_t q[16];
+                float v[16], next[16];
+                tmem_ld16(from + c, q);
+                residuals_of(a, o, token0 + c + 16u, n, live > c + 16u ? live - c - 16u : 0u, next);  // (asked for a round ahead)
+                tmem_ld_wait();
+#pragma unroll
+                for (uint32_t j = 0; j < 16u; ++j) {
+                    v[j] = __uint_as_float(q[j]);
+                }
+                finish(a, o, token0 + c, n, live - c, v, r);
+#pragma unroll
+                for (uint32_t j = 0; j < 16u; ++j) {
+                    r[j] = next[j];
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0u) {
+                asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
+                                 at_rank(base + S::ACC_EMPTY + 8 * b, 0))
+                             : "memory");
+            }
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    cluster_arrive();
+    cluster_wait();  // (neither block's barriers and tensor memory go while the other may use them)
+    tc_fence_after();
+    if (warp == 1u) {
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::COLS) : "memory");
     }
     if (tid == 0 && *abort_word) {
         atomicOr(a.status_word, 1u << lily_head::STATUS_TIMEOUT_BIT);
@@ -375,6 +669,26 @@ cudaError_t launch_few(const LinearArgs &a, uint32_t tiles, uint32_t shares, cud
     cfg.attrs = attr;
     cfg.numAttrs = 2;
     return cudaLaunchKernelEx(&cfg, linear_few_kernel<N, E4M3>, a);
+}
+
+template <bool E4M3>
+cudaError_t launch_many(const LinearArgs &a, uint32_t pairs, cudaStream_t stream) {
+    static std::atomic<uint64_t> ready{0};
+    const cudaError_t e = set_up(linear_many_kernel<E4M3>, Many::BYTES, ready);
+    if (e != cudaSuccess) {
+        return e;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2u * pairs, 1, 1);
+    cfg.blockDim = dim3(Many::THREADS, 1, 1);
+    cfg.dynamicSmemBytes = Many::BYTES;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, linear_many_kernel<E4M3>, a);
 }
 
 template <bool E4M3>
@@ -460,6 +774,18 @@ extern "C" int32_t lily_linear(lily_sampler_t *h, void *stream_, const lily_line
     a.lost_stage = h->lost_stage;
     h->lost_stage = 0xFFFFFFFFu;  // one launch only
 
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+    const uint64_t big_tiles = (uint64_t)((g.tokens + Many::TILE - 1u) / Many::TILE) * ((g.outputs + Many::TILE - 1u) / Many::TILE);
+    if (g.tokens > 256u && big_tiles <= 0x7FFFFFFFull) {
+        if (!encode_rows(&a.w_map, g.weight, g.weight_ld, g.outputs, g.columns, g.dtype, TILE_M) ||
+            !encode_rows(&a.a_map, g.a, g.a_ld, g.tokens, g.columns, g.dtype, TILE_M)) {
+            return fail(h, LILY_ERR_CUDA, "cuTensorMapEncodeTiled refused a or weight");
+        }
+        a.token_tiles = (g.tokens + Many::TILE - 1u) / Many::TILE;
+        const uint32_t pairs = (uint32_t)std::min<uint64_t>(big_tiles, (uint32_t)h->sm_count / 2u);
+        CU(h, e4m3 ? launch_many<true>(a, pairs, stream) : launch_many<false>(a, pairs, stream));
+        return LILY_OK;
+    }
     const uint32_t n = g.tokens <= 16u ? 16u : g.tokens <= 32u ? 32u : g.tokens <= 64u ? 64u : 128u;
     if (!encode_rows(&a.w_map, g.weight, g.weight_ld, g.outputs, g.columns, g.dtype, TILE_M) ||
         !encode_rows(&a.a_map, g.a, g.a_ld, g.tokens, g.columns, g.dtype, n)) {
@@ -476,7 +802,6 @@ extern "C" int32_t lily_linear(lily_sampler_t *h, void *stream_, const lily_line
     while (shares > 1u && (tiles * shares > room || a.blocks < 4u * shares)) {
         shares /= 2u;
     }
-    cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     CU(h, e4m3 ? few_by_tokens<true>(a, n, (uint32_t)tiles, shares, stream)
                : few_by_tokens<false>(a, n, (uint32_t)tiles, shares, stream));
     return LILY_OK;
