@@ -1,11 +1,16 @@
 // Biases, penalties, bans and grammar masks written onto logits (lily_adjust_logits,
 // include/lily_sampler.h).
 //
-// A row is cut into slices of the vocabulary, a block each. A block marks in shared memory what the
-// row's lists say about its own ids (the whole lists are read by every slice: they come out of L2),
-// then passes over its logits once. Blocks have nothing to say to one another, so nothing is kept
-// between calls and no workspace is needed. A logit that the mask takes away is not read, and in
-// place one that nothing changes is neither read nor written.
+// Masks and bans alone are one pass over the logits: mask_logits_kernel. A logit that goes is not
+// read, and in place one that stays is neither read nor written.
+//
+// Penalties and biases change a few thousand ids of a row, which the row's lists name: adjust_logits_kernel. A row
+// is cut into slices of the vocabulary (where there are few rows; a large batch's rows are a block each),
+// whose blocks' halves work side by side: the first passes over the slice's logits as above, the second
+// marks the ids of the slice that the history has, a bit each, numbers them (a prefix sum over the bits), and
+// reads the history again to count them by their numbers: a few thousand counts instead of one for every
+// id. When both are done, the numbered ids, which lie evenly on the threads, are penalised. Blocks have nothing
+// to say to one another, so nothing is kept between calls and no workspace is needed.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -20,9 +25,8 @@ namespace {
 
 using namespace lily_host;
 
-constexpr uint32_t NT = 512;
-constexpr uint32_t MOST_SMEM = 100u * 1024u;  // of a block: two on an SM
-constexpr uint32_t NO_SLOT = 0xFFFFFFFFu;
+constexpr uint32_t NO_SLOT = 0xFFFFFFFFu, NONE = 0xFFFFFFFFu, FULL = 0xFFFFFFFFu;
+constexpr uint32_t MAX_LIST = 512;  // the most that a handle's max_list can be
 
 struct RowPenalty {
     float repetition, presence, frequency;
@@ -34,7 +38,7 @@ struct AdjustArgs {
     void *out;
     uint64_t logits_ld, out_ld;
     const lily_sampling_params_t *params;  // on the device, or null
-    const uint32_t *history_ids, *history_len;
+    const uint32_t *history_ids, *history_len;  // (ids null: no row of the call has penalties)
     const uint32_t *bias_ids, *bias_len;
     const float *bias_vals;
     const uint32_t *ban_ids, *ban_len;
@@ -44,10 +48,12 @@ struct AdjustArgs {
     const uint32_t *counts_table, *seen_table;
     uint32_t seen_words;
     uint32_t *out_status, *status_word;
-    uint32_t row0, vocab, first_id, slice_len, masks, max_history, max_list;
+    uint32_t row0, rows, tasks;  // a launch's rows; rows x slices
+    uint32_t vocab, first_id, slice_len, masks, max_history, max_list;
     uint32_t in_place;
-    uint32_t wide_counts;   // 32 bits a count: lists that can hold an id more than 65535 times
-    uint32_t room_counts;   // whether the block has room for counts at all
+    // A block's shared memory, in words from its start: bits of the ids that stay, of those in the history, how
+    // many of those there are before each word of bits.
+    uint32_t seen_at, before_at, direct;  // (the latter two words if not `direct`: see the kernel)
 };
 
 // The penalties of a launch's rows travel in its arguments.
@@ -59,68 +65,16 @@ struct AdjustLaunch {
 
 __device__ __forceinline__ float neg_inf() { return __uint_as_float(0xFF800000u); }
 
-// What the block's shared memory says about an id of its slice.
-struct Marks {
-    const uint32_t *seen, *biased, *banned;
-    const void *counts;
-};
-
-// A row as its block sees it.
-struct Row {
-    float repetition, presence, frequency;
-    bool penalties, counted, listed_bias, listed_ban;
-    const uint32_t *slot_seen, *slot_counts;  // the histogram slot's, from the slice's first id on
-    const uint32_t *bias_ids;
-    const float *bias_vals;
-    uint32_t bias_len;
-    const uint32_t *mask;   // the row's words, or null
-    uint32_t id0;           // global id of the slice's first logit
-};
-
-// The 32 bits of a row of words from bit `bit` on; only words that hold one of the `n` wanted bits are read.
-__device__ __forceinline__ uint32_t bits_at(const uint32_t *words, uint32_t bit, uint32_t n) {
-    const uint32_t w = bit / 32u, s = bit % 32u;
+// `n` bits (at most 32) of a row of words from bit `bit` on, which may lie up to 7 before its first; only
+// words that hold one of them are read. What is beyond them is not defined.
+__device__ __forceinline__ uint32_t bits_at(const uint32_t *words, int32_t bit, uint32_t n) {
+    if (bit < 0) {
+        return __ldg(words) << -bit;
+    }
+    const uint32_t w = (uint32_t)bit / 32u, s = (uint32_t)bit % 32u;
     const uint32_t lo = __ldg(words + w);
     const uint32_t hi = s + n > 32u ? __ldg(words + w + 1u) : 0u;
     return __funnelshift_r(lo, hi, s);
-}
-
-__device__ __forceinline__ uint32_t count_of(const AdjustArgs &a, const Marks &m, const Row &r, uint32_t at) {
-    if (r.slot_seen != nullptr) {
-        return __ldg(r.slot_counts + at);
-    }
-    return a.wide_counts ? static_cast<const uint32_t *>(m.counts)[at] : static_cast<const uint16_t *>(m.counts)[at];
-}
-
-// Logit `x` of place `at` of the slice, biased and penalised as the marks say.
-__device__ __forceinline__ float adjusted(const AdjustArgs &a, const Marks &m, const Row &r, uint32_t at, float x,
-                                          bool seen, bool biased) {
-    if (biased) {
-        for (uint32_t j = 0; j < r.bias_len; ++j) {
-            if (__ldg(r.bias_ids + j) == r.id0 + at) {
-                x = __fadd_rn(x, __ldg(r.bias_vals + j));
-            }
-        }
-    }
-    if (seen) {
-        const float count = r.counted ? (float)count_of(a, m, r, at) : 1.0f;
-        if (count > 0.0f) {
-            x = x > 0.0f ? __fdiv_rn(x, r.repetition) : __fmul_rn(x, r.repetition);
-            x = __fsub_rn(x, __fadd_rn(r.presence, __fmul_rn(r.frequency, count)));
-        }
-    }
-    return x;
-}
-
-// Which of the 32 ids of word `w` of the slice have been seen, biased, and may be drawn; n of them exist.
-__device__ __forceinline__ void words_of(const Marks &m, const Row &r, uint32_t w, uint32_t n, uint32_t &seen,
-                                         uint32_t &biased, uint32_t &allowed) {
-    seen = !r.penalties ? 0u : r.slot_seen != nullptr ? __ldg(r.slot_seen + w) : m.seen[w];
-    biased = r.listed_bias ? m.biased[w] : 0u;
-    allowed = r.mask != nullptr ? bits_at(r.mask, r.id0 + w * 32u, n) : 0xFFFFFFFFu;
-    if (r.listed_ban) {
-        allowed &= ~m.banned[w];
-    }
 }
 
 __device__ __forceinline__ float widen(float f) { return f; }
@@ -133,299 +87,575 @@ template <typename T>
 struct Raw;
 template <>
 struct Raw<float> {
-    float4 a, b;
+    uint4 q[2];
 };
 template <>
 struct Raw<__nv_bfloat16> {
-    uint4 q;
+    uint4 q[1];
 };
 
-__device__ __forceinline__ void load8(const float *p, Raw<float> &r) {
-    r.a = __ldcs(reinterpret_cast<const float4 *>(p)), r.b = __ldcs(reinterpret_cast<const float4 *>(p) + 1);
-}
-__device__ __forceinline__ void load8(const __nv_bfloat16 *p, Raw<__nv_bfloat16> &r) {
-    r.q = __ldcs(reinterpret_cast<const uint4 *>(p));
-}
-
-__device__ __forceinline__ void unpack(const Raw<float> &r, float (&f)[8]) {
-    f[0] = r.a.x, f[1] = r.a.y, f[2] = r.a.z, f[3] = r.a.w, f[4] = r.b.x, f[5] = r.b.y, f[6] = r.b.z, f[7] = r.b.w;
-}
-__device__ __forceinline__ void unpack(const Raw<__nv_bfloat16> &r, float (&f)[8]) {
-    const uint32_t w[4] = {r.q.x, r.q.y, r.q.z, r.q.w};
+template <typename T>
+__device__ __forceinline__ void load8(const T *p, Raw<T> &r) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        f[2 * i] = __uint_as_float(w[i] << 16);
-        f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    for (uint32_t i = 0; i < sizeof(T) / 2u; ++i) {
+        r.q[i] = __ldcs(reinterpret_cast<const uint4 *>(p) + i);
     }
 }
 
-__device__ __forceinline__ void store8(float *p, const float (&f)[8]) {
-    reinterpret_cast<float4 *>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
-    reinterpret_cast<float4 *>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+__device__ __forceinline__ uint32_t masked(uint32_t two, uint32_t keep) {  // two bf16, by the two lowest bits of `keep`
+    two = keep & 1u ? two : (two & 0xFFFF0000u) | 0xFF80u;
+    return keep & 2u ? two : (two & 0xFFFFu) | 0xFF800000u;
 }
 
-__device__ __forceinline__ void store8(__nv_bfloat16 *p, const float (&f)[8]) {
-    uint32_t w[4];
+// Eight logits written, -inf where `keep` has no bit.
+__device__ __forceinline__ void store8(float *p, const Raw<float> &r, uint32_t keep) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const __nv_bfloat162 b = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
-        w[i] = *reinterpret_cast<const uint32_t *>(&b);
+    for (uint32_t i = 0; i < 2u; ++i) {
+        uint4 q = r.q[i];
+        const uint32_t k = keep >> (4u * i);
+        q.x = k & 1u ? q.x : 0xFF800000u, q.y = k & 2u ? q.y : 0xFF800000u;
+        q.z = k & 4u ? q.z : 0xFF800000u, q.w = k & 8u ? q.w : 0xFF800000u;
+        reinterpret_cast<uint4 *>(p)[i] = q;
     }
-    *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ void store8(__nv_bfloat16 *p, const Raw<__nv_bfloat16> &r, uint32_t keep) {
+    uint4 q = r.q[0];
+    if (keep != 0xFFu) {
+        q = make_uint4(masked(q.x, keep), masked(q.y, keep >> 2), masked(q.z, keep >> 4), masked(q.w, keep >> 6));
+    }
+    *reinterpret_cast<uint4 *>(p) = q;
+}
+__device__ __forceinline__ void store8(float *p, const Raw<__nv_bfloat16> &r, uint32_t keep) {
+    const uint32_t w[4] = {r.q[0].x, r.q[0].y, r.q[0].z, r.q[0].w};
+    Raw<float> f;
+#pragma unroll
+    for (uint32_t i = 0; i < 2u; ++i) {
+        f.q[i] = make_uint4(w[2 * i] << 16, w[2 * i] & 0xFFFF0000u, w[2 * i + 1] << 16, w[2 * i + 1] & 0xFFFF0000u);
+    }
+    store8(p, f, keep);
 }
 
-// What the row's lists say about the slice, into shared memory (cleared before).
-__device__ __forceinline__ void mark(uint32_t *words, uint32_t at) { atomicOr(words + at / 32u, 1u << (at % 32u)); }
+// A row's history as a slice's block reads it: all of it. base: the id of place 0; the slice's are the `n`
+// places from `shift` on.
+struct HistoryList {
+    const uint32_t *ids;
+    uint32_t length, base, shift, n;
 
-// TI: the logits' type, TO: out's. WIDE: rows start on 16-byte boundaries in both.
-template <typename TI, typename TO, bool WIDE, uint32_t MAX_ROWS>
-__global__ void __launch_bounds__(NT, 2) adjust_logits_kernel(const __grid_constant__ AdjustLaunch<MAX_ROWS> l) {
+    // f(eight places, NONE for those that are not the slice's) over the list, by the warps of a block that
+    // come here, whenever they do: they take the list's parts in turn (`next`, in shared memory, from 0), the
+    // next one's ids asked for before one's are looked at.
+    template <typename F>
+    __device__ __forceinline__ void each(uint32_t *next, F f) const {
+        constexpr uint32_t AHEAD = 4u;  // vectors of a lane in a part
+        const uint32_t lane = threadIdx.x % 32u;
+        const uint32_t head = min(length, (uint32_t)((16u - (reinterpret_cast<uintptr_t>(ids) & 15u)) & 15u) / 4u);
+        const uint32_t quads = (length - head) / 4u, parts = (quads + 32u * AHEAD - 1u) / (32u * AHEAD);
+        const uint4 *four = reinterpret_cast<const uint4 *>(ids + head);
+        const auto place = [&](uint32_t id) { return id - base - shift < n ? id - base : NONE; };  // (an id below the slice wraps around)
+        uint4 v[AHEAD];
+        const auto take = [&]() {
+            uint32_t part = 0;
+            if (lane == 0u) {
+                part = atomicAdd(next, 1u);
+            }
+            part = __shfl_sync(FULL, part, 0);
+#pragma unroll
+            for (uint32_t k = 0; k < AHEAD; ++k) {
+                const uint32_t q = (part * AHEAD + k) * 32u + lane;
+                v[k] = q < quads ? __ldg(four + q) : make_uint4(NONE, NONE, NONE, NONE);
+            }
+            return part;
+        };
+        uint32_t part = take();
+        while (part < parts) {
+            uint32_t p[AHEAD][4];
+#pragma unroll
+            for (uint32_t k = 0; k < AHEAD; ++k) {
+                p[k][0] = place(v[k].x), p[k][1] = place(v[k].y), p[k][2] = place(v[k].z), p[k][3] = place(v[k].w);
+            }
+            part = take();
+#pragma unroll
+            for (uint32_t k = 0; k < AHEAD; k += 2u) {
+                const uint32_t eight[8] = {p[k][0], p[k][1], p[k][2], p[k][3], p[k + 1u][0], p[k + 1u][1], p[k + 1u][2], p[k + 1u][3]};
+                f(eight);
+            }
+        }
+        if (part == parts) {  // one warp: up to three ids in front, up to three behind
+            const uint32_t behind = head + 4u * quads + lane - 4u;
+            const uint32_t id = lane < head ? __ldg(ids + lane) : lane >= 4u && behind < length ? __ldg(ids + behind) : NONE;
+            const uint32_t eight[8] = {place(id), NONE, NONE, NONE, NONE, NONE, NONE, NONE};
+            f(eight);
+        }
+    }
+};
+
+// Barriers of parts of a block (`threads`: those that arrive and those that wait).
+constexpr uint32_t BAR_ALL = 0, BAR_STREAM = 1, BAR_LISTS = 2;
+__device__ __forceinline__ void bar_sync(uint32_t bar, uint32_t threads) {
+    asm volatile("bar.sync %0, %1;" ::"r"(bar), "r"(threads) : "memory");
+}
+// A task: a row's slice. WIDE: rows of logits and out start on boundaries of eight logits, or miss one
+// by as much; a slice's places are then counted from the boundary before its first logit (`shift` places
+// earlier), so that eight logits of a boundary are eight marks of one.
+template <typename TI, typename TO, bool WIDE>
+struct Task {
+    const TI *from;
+    TO *to;
+    const uint32_t *mask;  // the row's words, or null
+    float repetition, presence, frequency;
+    uint32_t row, slot, history, bias_len, ban_len;
+    uint32_t lo, n, id0, shift;  // the slice's first logit, its length, its first id
+    uint32_t words;              // of bits, of a slice
+    bool fine, penalties;
+
+    template <uint32_t MAX_ROWS>
+    __device__ __forceinline__ Task(const AdjustLaunch<MAX_ROWS> &l, uint32_t task) {
+        const AdjustArgs &a = l.a;
+        const uint32_t at = task % a.rows, slice = task / a.rows;
+        row = a.row0 + at;
+        lo = slice * a.slice_len, n = min(a.slice_len, a.vocab - lo);
+        words = a.slice_len / 32u + 8u;  // (slices are multiples of 256 ids)
+        uint32_t status = LILY_ROW_OK;
+        slot = NO_SLOT, repetition = 1.0f, presence = 0.0f, frequency = 0.0f;
+        if (a.params != nullptr) {
+            const lily_sampling_params_t &p = a.params[row];
+            repetition = p.repetition_penalty, presence = p.presence_penalty, frequency = p.frequency_penalty;
+            const bool valid = isfinite(p.temperature) && p.temperature >= 0.0f && isfinite(p.top_p) && p.top_p > 0.0f &&
+                               p.top_p <= 1.0f && isfinite(p.min_p) && p.min_p >= 0.0f && p.min_p <= 1.0f &&
+                               isfinite(repetition) && repetition > 0.0f && isfinite(presence) && isfinite(frequency);
+            status = valid ? status : LILY_ROW_PARAMS;
+        }
+        if (MAX_ROWS > 1u) {
+            const RowPenalty &p = l.rows[at];
+            slot = p.slot;
+            if (a.params == nullptr) {
+                repetition = p.repetition, presence = p.presence, frequency = p.frequency;
+            }
+        }
+        penalties = presence != 0.0f || frequency != 0.0f || repetition != 1.0f;
+        history = bias_len = ban_len = 0u;
+        if (a.history_len != nullptr && slot == NO_SLOT) {
+            history = a.history_len[row];
+            status = history > a.max_history || history > a.history_ld ? LILY_ROW_LIST : status;
+        }
+        if (a.bias_ids != nullptr) {
+            bias_len = a.bias_len[row];
+            status = bias_len > a.max_list || bias_len > a.bias_ld ? LILY_ROW_LIST : status;
+        }
+        if (a.ban_ids != nullptr) {
+            ban_len = a.ban_len[row];
+            status = ban_len > a.max_list || ban_len > a.ban_ld ? LILY_ROW_LIST : status;
+        }
+        const int32_t mask_row = a.mask != nullptr ? (a.mask_rows != nullptr ? a.mask_rows[row] : (int32_t)row) : -1;
+        status = mask_row >= 0 && (uint32_t)mask_row >= a.masks ? LILY_ROW_LIST : status;
+        mask = mask_row >= 0 ? a.mask + (uint64_t)mask_row * a.mask_ld : nullptr;
+        fine = status == LILY_ROW_OK;
+        if (slice == 0u && threadIdx.x == 0u) {
+            if (a.out_status != nullptr) {
+                a.out_status[row] = status;
+            }
+            if (!fine) {
+                atomicOr(a.status_word, 1u << status);
+            }
+        }
+        history = penalties && fine && a.history_ids != nullptr ? history : 0u;
+        bias_len = fine ? bias_len : 0u;
+        id0 = a.first_id + lo;
+        from = static_cast<const TI *>(a.logits) + (uint64_t)row * a.logits_ld + lo;
+        to = static_cast<TO *>(a.out) + (uint64_t)row * a.out_ld + lo;
+        shift = WIDE ? (uint32_t)(reinterpret_cast<uintptr_t>(from) / sizeof(TI)) % 8u : 0u;
+    }
+
+    __device__ __forceinline__ bool from_slot() const { return fine && penalties && slot != NO_SLOT; }
+    __device__ __forceinline__ bool masks() const { return mask != nullptr || ban_len > 0u; }
+    __device__ __forceinline__ bool keeps() const { return masks() || bias_len > 0u; }
+    // Vectors of eight places; the first and the last may have fewer.
+    __device__ __forceinline__ uint32_t chunks() const { return (n + shift + 7u) / 8u; }
+    // Of the eight places from 8 c on, those that stay.
+    __device__ __forceinline__ uint32_t stay8(const uint32_t *kept, uint32_t c) const {
+        return keeps() ? (uint32_t)reinterpret_cast<const uint8_t *>(kept)[c] : 0xFFu;
+    }
+
+    // The slice's logits, masked and written, by `width` threads of which this is number t; what stays goes
+    // into `kept`, a bit each (if anything goes, or biases have ids to take out).
+    __device__ __forceinline__ void stream(const AdjustArgs &a, uint32_t *kept, uint32_t t, uint32_t width) const {
+        if (keeps()) {
+            if (ban_len > 0u) {
+                for (uint32_t i = t; i < words; i += width) {
+                    kept[i] = 0u;
+                }
+                bar_sync(BAR_STREAM, width);
+                for (uint32_t j = t; j < ban_len; j += width) {
+                    const uint32_t at = __ldg(a.ban_ids + (uint64_t)row * a.ban_ld + j) - id0;
+                    if (at < n) {
+                        atomicOr(kept + (at + shift) / 32u, 1u << ((at + shift) % 32u));
+                    }
+                }
+                bar_sync(BAR_STREAM, width);
+            }
+            for (uint32_t i = t; i * 32u < n + shift; i += width) {
+                const int32_t first = (int32_t)(i * 32u) - (int32_t)shift;
+                const uint32_t stay =
+                    mask != nullptr ? bits_at(mask, (int32_t)id0 + first, min(32u, (uint32_t)((int32_t)n - first))) : FULL;
+                kept[i] = ban_len > 0u ? stay & ~kept[i] : stay;
+            }
+            bar_sync(BAR_STREAM, width);
+        }
+        if (a.in_place && !masks()) {
+            return;
+        }
+        if (!WIDE) {
+            for (uint32_t c = t; c < chunks(); c += width) {
+                one_by_one(a, kept, c);
+            }
+            return;
+        }
+        const uint32_t begin = shift != 0u ? 1u : 0u, end = (n + shift) / 8u;  // the whole vectors
+        const TI *from8 = from - shift;
+        TO *to8 = to - shift;
+        constexpr uint32_t AHEAD = sizeof(TI) == 2 ? 8u : 4u;
+        for (uint32_t c = begin + t; c < end; c += width * AHEAD) {
+            Raw<TI> raw[AHEAD];
+            uint32_t keeps[AHEAD / 4u];  // a byte each
+#pragma unroll
+            for (uint32_t k = 0; k < AHEAD; ++k) {
+                const uint32_t keep = c + k * width < end ? stay8(kept, c + k * width) : 0u;
+                keeps[k / 4u] = k % 4u ? keeps[k / 4u] | keep << k % 4u * 8u : keep;
+                if (keep != 0u && !(a.in_place && keep == 0xFFu)) {
+                    load8(from8 + (c + k * width) * 8u, raw[k]);
+                }
+            }
+#pragma unroll
+            for (uint32_t k = 0; k < AHEAD; ++k) {
+                const uint32_t keep = keeps[k / 4u] >> k % 4u * 8u & 0xFFu;
+                if (c + k * width < end && !(a.in_place && keep == 0xFFu)) {
+                    store8(to8 + (c + k * width) * 8u, raw[k], keep);
+                }
+            }
+        }
+        if (t == 0u && begin != 0u) {
+            one_by_one(a, kept, 0u);
+        }
+        if (t == width - 1u && end < chunks() && (end != 0u || begin == 0u)) {
+            one_by_one(a, kept, end);
+        }
+    }
+
+private:
+    // A vector that is not whole, or whose logits and outs do not lie alike.
+    __device__ __forceinline__ void one_by_one(const AdjustArgs &a, const uint32_t *kept, uint32_t c) const {
+        const int32_t first = (int32_t)(c * 8u) - (int32_t)shift;
+        const uint32_t keep = stay8(kept, c);
+        for (int32_t i = 0; i < 8; ++i) {
+            if (first + i >= 0 && first + i < (int32_t)n) {
+                if (!(keep >> i & 1u)) {
+                    narrow(to + first + i, neg_inf());
+                } else if (!a.in_place) {
+                    narrow(to + first + i, widen(from[first + i]));
+                }
+            }
+        }
+    }
+};
+
+constexpr uint32_t MASK_NT = 512;
+
+// Masks and bans alone. Grid: rows x slices.
+template <typename TI, typename TO, bool WIDE>
+__global__ void __launch_bounds__(MASK_NT, 2) mask_logits_kernel(const __grid_constant__ AdjustLaunch<1> l) {
     extern __shared__ __align__(16) uint32_t smem[];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const AdjustArgs &a = l.a;
-    const uint32_t t = threadIdx.x, row = a.row0 + blockIdx.y;
-    const uint32_t lo = blockIdx.x * a.slice_len, n = min(a.slice_len, a.vocab - lo);
+    const Task<TI, TO, WIDE> task(l, blockIdx.x);
+    if (task.fine) {
+        task.stream(l.a, smem, threadIdx.x, MASK_NT);
+    }
+}
 
-    // The row's parameters and lengths, and whether they are in order.
-    Row r;
-    uint32_t slot = NO_SLOT, status = LILY_ROW_OK;
-    r.repetition = 1.0f, r.presence = 0.0f, r.frequency = 0.0f;
-    if (a.params != nullptr) {
-        const lily_sampling_params_t &p = a.params[row];
-        r.repetition = p.repetition_penalty, r.presence = p.presence_penalty, r.frequency = p.frequency_penalty;
-        const bool fine = isfinite(p.temperature) && p.temperature >= 0.0f && isfinite(p.top_p) && p.top_p > 0.0f &&
-                          p.top_p <= 1.0f && isfinite(p.min_p) && p.min_p >= 0.0f && p.min_p <= 1.0f &&
-                          isfinite(r.repetition) && r.repetition > 0.0f && isfinite(r.presence) && isfinite(r.frequency);
-        status = fine ? status : LILY_ROW_PARAMS;
-    }
-    if (MAX_ROWS > 1u) {
-        const RowPenalty &p = l.rows[blockIdx.y];
-        slot = p.slot;
-        if (a.params == nullptr) {
-            r.repetition = p.repetition, r.presence = p.presence, r.frequency = p.frequency;
-        }
-    }
-    r.penalties = r.presence != 0.0f || r.frequency != 0.0f || r.repetition != 1.0f;
-    uint32_t history = 0, ban_len = 0;
-    r.bias_len = 0;
-    if (a.history_ids != nullptr && slot == NO_SLOT) {
-        history = a.history_len[row];
-        status = history > a.max_history || history > a.history_ld ? LILY_ROW_LIST : status;
-    }
-    if (a.bias_ids != nullptr) {
-        r.bias_len = a.bias_len[row];
-        status = r.bias_len > a.max_list || r.bias_len > a.bias_ld ? LILY_ROW_LIST : status;
-    }
-    if (a.ban_ids != nullptr) {
-        ban_len = a.ban_len[row];
-        status = ban_len > a.max_list || ban_len > a.ban_ld ? LILY_ROW_LIST : status;
-    }
-    int32_t mask_row = a.mask != nullptr ? (a.mask_rows != nullptr ? a.mask_rows[row] : (int32_t)row) : -1;
-    status = mask_row >= 0 && (uint32_t)mask_row >= a.masks ? LILY_ROW_LIST : status;
-    if (blockIdx.x == 0u && t == 0u) {
-        if (a.out_status != nullptr) {
-            a.out_status[row] = status;
-        }
-        if (status != LILY_ROW_OK) {
-            atomicOr(a.status_word, 1u << status);
-        }
-    }
-    if (status != LILY_ROW_OK) {
+constexpr uint32_t NT = 512, HALF = NT / 2;
+constexpr uint32_t WINDOW = 5120;  // numbered ids that a block counts at a time
+
+// Grid: rows x slices, the rows' first slices first.
+template <typename TI, typename TO, bool WIDE, uint32_t MAX_ROWS>
+__global__ void __launch_bounds__(NT, 2) adjust_logits_kernel(const __grid_constant__ AdjustLaunch<MAX_ROWS> l) {
+    extern __shared__ __align__(16) uint32_t smem[];
+    __shared__ uint32_t window[2u * WINDOW], sums[NT / 32u], next_part, bias_id[MAX_LIST];
+    __shared__ float bias_val[MAX_LIST];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const AdjustArgs &a = l.a;
+    const Task<TI, TO, WIDE> task(l, blockIdx.x);
+    if (!task.fine) {
         return;
     }
-    history = r.penalties ? history : 0u;
-    r.penalties = r.penalties && (history > 0u || slot != NO_SLOT);
-    r.counted = slot != NO_SLOT || r.frequency != 0.0f;
-    r.listed_bias = r.bias_len > 0u;
-    r.listed_ban = ban_len > 0u;
-    r.id0 = a.first_id + lo;
-    r.mask = mask_row >= 0 ? a.mask + (uint64_t)mask_row * a.mask_ld : nullptr;
-    r.bias_ids = a.bias_ids + (uint64_t)row * a.bias_ld;
-    r.bias_vals = a.bias_vals + (uint64_t)row * a.bias_ld;
-    r.slot_seen = r.slot_counts = nullptr;
-    if (slot != NO_SLOT) {
-        r.slot_seen = a.seen_table + (uint64_t)slot * a.seen_words + lo / 32u;
-        r.slot_counts = a.counts_table + (uint64_t)slot * a.vocab + lo;
-    }
+    uint32_t *kept = smem, *seen = smem + a.seen_at, *before = smem + a.before_at;
+    // A slice no longer than two windows needs no numbers: its places are counted as they are; so are those of
+    // one of four windows, in 16 bits, if no list can have an id more often than they hold.
+    const bool direct = a.direct != 0u, halves = a.direct == 2u;
+    uint32_t *count_of = window, *place_of = window + WINDOW;
+    const uint32_t t = threadIdx.x, lane = t % 32u, shift = task.shift;
+    const uint32_t units = (task.n + shift + 31u) / 32u;  // words of bits
+    const bool from_slot = task.from_slot(), history = task.history > 0u;
 
-    // Marks: three words of bits per 32 ids, then the counts of a row with a frequency penalty.
-    const uint32_t words = a.slice_len / 32u;
-    uint32_t *seen = smem, *biased = smem + words, *banned = smem + 2u * words, *counts = smem + 3u * words;
-    const bool own_counts = history > 0u && r.counted;
-    const bool marks = history > 0u || r.listed_bias || r.listed_ban;
-    if (marks) {
-        const uint32_t clear = 3u * words + (own_counts ? (a.wide_counts ? a.slice_len : a.slice_len / 2u) : 0u);
-        for (uint32_t i = t * 4u; i < clear; i += NT * 4u) {  // (slices are multiples of 256 ids)
-            *reinterpret_cast<uint4 *>(smem + i) = make_uint4(0u, 0u, 0u, 0u);
+    // The second half finds out what the lists say while the first one passes over the logits; where a
+    // short slice has a long history, both see to that together afterwards.
+    const bool together = task.history > 2u * task.n;
+    if (t < HALF) {
+        task.stream(a, kept, t, HALF);
+    } else {
+        for (uint32_t i = t - HALF; history && i < (halves ? units * 16u : direct ? task.n + shift : units); i += HALF) {
+            (direct ? count_of : seen)[i] = 0u;
         }
+        for (uint32_t j = t - HALF; j < task.bias_len; j += HALF) {
+            bias_id[j] = __ldg(a.bias_ids + (uint64_t)task.row * a.bias_ld + j);
+            bias_val[j] = __ldg(a.bias_vals + (uint64_t)task.row * a.bias_ld + j);
+        }
+        if (t == HALF) {
+            next_part = 0u;
+        }
+    }
+    if (together) {
         __syncthreads();
-        const uint32_t *ids = a.history_ids + (uint64_t)row * a.history_ld;
-        const auto mark_history = [&](uint32_t id) {
-            const uint32_t at = id - r.id0;  // (ids below the slice wrap around)
-            if (at < n) {
-                mark(seen, at);
-                if (own_counts) {
-                    if (a.wide_counts) {
-                        atomicAdd(counts + at, 1u);
+    }
+    const uint32_t width = together ? NT : HALF, bar = together ? BAR_ALL : BAR_LISTS, me = together ? t : t - HALF;
+    const HistoryList ids{a.history_ids + (uint64_t)task.row * a.history_ld, task.history, task.id0 - shift, shift, task.n};
+    const auto mark_and_number = [&]() {
+        ids.each(&next_part, [&](const uint32_t (&place)[8]) {
+            // (Looked at first, all eight together: an or on a word that most of a warp means takes turns.)
+            uint32_t word[8];
+#pragma unroll
+            for (uint32_t k = 0; k < 8u; ++k) {
+                word[k] = place[k] != NONE ? reinterpret_cast<volatile uint32_t *>(seen)[place[k] / 32u] : 0xFFFFFFFFu;
+            }
+#pragma unroll
+            for (uint32_t k = 0; k < 8u; ++k) {
+                if (!(word[k] >> place[k] % 32u & 1u)) {
+                    atomicOr(seen + place[k] / 32u, 1u << place[k] % 32u);
+                }
+            }
+        });
+        bar_sync(bar, width);
+        // ---- numbered: what is before each word. A thread adds up neighbours.
+        const uint32_t each = (units + width - 1u) / width | 1u, first = me * each;
+        uint32_t mine = 0;
+        for (uint32_t i = 0; i < each; ++i) {
+            mine += first + i < units ? (uint32_t)__popc(seen[first + i]) : 0u;
+        }
+        uint32_t upto = mine;
+#pragma unroll
+        for (uint32_t o = 1; o < 32u; o *= 2u) {
+            const uint32_t below = __shfl_up_sync(FULL, upto, o);
+            upto += lane >= o ? below : 0u;
+        }
+        if (lane == 31u) {
+            sums[me / 32u] = upto;
+        }
+        if (me == 0u) {
+            next_part = 0u;
+        }
+        bar_sync(bar, width);
+        uint32_t warps = lane < width / 32u ? sums[lane] : 0u;
+#pragma unroll
+        for (uint32_t o = 1; o < 32u; o *= 2u) {
+            const uint32_t below = __shfl_up_sync(FULL, warps, o);
+            warps += lane >= o ? below : 0u;
+        }
+        uint32_t at = upto - mine + (me >= 32u ? __shfl_sync(FULL, warps, (me / 32u + 31u) % 32u) : 0u);
+        for (uint32_t i = 0; i < each && first + i < units; ++i) {
+            before[first + i] = at;
+            at += (uint32_t)__popc(seen[first + i]);
+        }
+        bar_sync(bar, width);
+    };
+    if (history && (together || t >= HALF)) {
+        bar_sync(bar, width);
+        // ---- the history's ids, a bit each (or their counts at once)
+        if (direct) {
+            ids.each(&next_part, [&](const uint32_t (&place)[8]) {
+#pragma unroll
+                for (uint32_t k = 0; k < 8u; ++k) {
+                    if (place[k] == NONE) {
+                    } else if (halves) {
+                        atomicAdd(count_of + place[k] / 2u, place[k] % 2u ? 0x10000u : 1u);
                     } else {
-                        atomicAdd(counts + at / 2u, at % 2u ? 0x10000u : 1u);
+                        atomicAdd(count_of + place[k], 1u);
+                    }
+                }
+            });
+        } else {
+            mark_and_number();
+        }
+    }
+    // Window by window (there is hardly ever a second one): the places of the numbers from `base` on, and how
+    // often they come.
+    const auto fill = [&](uint32_t base, uint32_t me, uint32_t width, uint32_t bar) {
+        for (uint32_t i = me; i < WINDOW; i += width) {
+            count_of[i] = 0u;
+        }
+        // (A warp's lanes look far apart: where ids are frequent, all of their neighbours are seen.)
+        const uint32_t apart = (units + 31u) / 32u | 1u;
+        for (uint32_t w = me / 32u; w < apart; w += width / 32u) {
+            const uint32_t u = lane * apart + w;
+            if (u < units) {
+                uint32_t at = before[u] - base;  // (wraps around where the window begins later)
+                for (uint32_t m = seen[u]; m != 0u; m &= m - 1u, ++at) {
+                    if (at < WINDOW) {
+                        place_of[at] = u * 32u + (uint32_t)__ffs(m) - 1u;
                     }
                 }
             }
-        };
-        const uint32_t head = min(history, (uint32_t)((16u - (reinterpret_cast<uintptr_t>(ids) & 15u)) & 15u) / 4u);
-        const uint32_t quads = (history - head) / 4u;
-        const uint4 *four = reinterpret_cast<const uint4 *>(ids + head);
-        for (uint32_t q = t; q < quads; q += NT * 4u) {
-            uint4 v[4];
+        }
+        bar_sync(bar, width);
+        if (task.frequency != 0.0f) {
+            ids.each(&next_part, [&](const uint32_t (&place)[8]) {
+                uint32_t at[8];
 #pragma unroll
-            for (uint32_t k = 0; k < 4u; ++k) {
-                if (q + k * NT < quads) {
-                    v[k] = __ldg(four + q + k * NT);
+                for (uint32_t k = 0; k < 8u; ++k) {
+                    const uint32_t u = place[k] / 32u;
+                    at[k] = place[k] != NONE ? before[u] + (uint32_t)__popc(seen[u] & ((1u << place[k] % 32u) - 1u)) - base : NONE;
                 }
-            }
 #pragma unroll
-            for (uint32_t k = 0; k < 4u; ++k) {
-                if (q + k * NT < quads) {
-                    mark_history(v[k].x), mark_history(v[k].y), mark_history(v[k].z), mark_history(v[k].w);
+                for (uint32_t k = 0; k < 8u; ++k) {
+                    if (at[k] < WINDOW) {
+                        atomicAdd(count_of + at[k], 1u);
+                    }
                 }
-            }
+            });
         }
-        if (t < head) {
-            mark_history(__ldg(ids + t));
-        }
-        if (head + 4u * quads + t < history) {
-            mark_history(__ldg(ids + head + 4u * quads + t));
-        }
-        for (uint32_t j = t; j < r.bias_len; j += NT) {
-            const uint32_t at = __ldg(r.bias_ids + j) - r.id0;
-            if (at < n) {
-                mark(biased, at);
-            }
-        }
-        const uint32_t *ban_ids = a.ban_ids + (uint64_t)row * a.ban_ld;
-        for (uint32_t j = t; j < ban_len; j += NT) {
-            const uint32_t at = __ldg(ban_ids + j) - r.id0;
-            if (at < n) {
-                mark(banned, at);
-            }
-        }
-        __syncthreads();
+    };
+    if (history && !direct && (together || t >= HALF)) {
+        fill(0u, me, width, bar);
     }
-    const Marks m = {seen, biased, banned, counts};
+    __syncthreads();  // (the logits are written, too)
+    const uint32_t total = !history ? 0u : direct ? task.n + shift : before[units - 1u] + (uint32_t)__popc(seen[units - 1u]);
 
-    const TI *from = static_cast<const TI *>(a.logits) + (uint64_t)row * a.logits_ld + lo;
-    TO *to = static_cast<TO *>(a.out) + (uint64_t)row * a.out_ld + lo;
-    if (WIDE) {
-        // A thread takes eight neighbours, a quarter of a word of marks, at a time.
-        constexpr uint32_t AHEAD = sizeof(TI) == 2 ? 4u : 2u;
-        const uint32_t chunks = n / 8u;
-        for (uint32_t c0 = t; c0 < chunks; c0 += NT * AHEAD) {
-            Raw<TI> raw[AHEAD];
-            uint32_t said[AHEAD];  // seen, biased, allowed, a byte each; bit 24: something is written
-#pragma unroll
-            for (uint32_t k = 0; k < AHEAD; ++k) {
-                const uint32_t c = c0 + k * NT;
-                said[k] = 0u;
-                if (c < chunks) {
-                    uint32_t s, b, w;
-                    const uint32_t word = c / 4u, shift = c % 4u * 8u;
-                    words_of(m, r, word, min(32u, n - word * 32u), s, b, w);
-                    s = (s >> shift) & 0xFFu, b = (b >> shift) & 0xFFu, w = (w >> shift) & 0xFFu;
-                    if (!a.in_place || w != 0xFFu || (s | b) != 0u) {
-                        said[k] = s | b << 8 | w << 16 | 1u << 24;
-                        if (w != 0u) {
-                            load8(from + c * 8u, raw[k]);
+    const auto counted = [&](uint32_t at) -> uint32_t {
+        return halves ? (uint32_t)reinterpret_cast<const uint16_t *>(count_of)[at] : count_of[at];
+    };
+
+    // ---- what the lists change
+    const uint32_t *slot_seen = a.seen_table + (from_slot ? (uint64_t)task.slot * a.seen_words : 0u);
+    const uint32_t *slot_counts = a.counts_table + (from_slot ? (uint64_t)task.slot * a.vocab : 0u) + task.lo;
+    const auto penalised = [&](float x, uint32_t count) {
+        x = x > 0.0f ? __fdiv_rn(x, task.repetition) : __fmul_rn(x, task.repetition);
+        return __fsub_rn(x, __fadd_rn(task.presence, __fmul_rn(task.frequency, (float)count)));
+    };
+    // A biased id is its first entry's, which adds up all of them in the list's order; its penalties follow
+    // where its count is known, and it no longer counts as one that stays.
+    for (uint32_t j = t; j < task.bias_len; j += NT) {
+        const uint32_t id = bias_id[j], in = id - task.id0, place = in + shift;
+        if (in >= task.n || !(kept[place / 32u] >> place % 32u & 1u)) {
+            continue;
+        }
+        bool first = true;
+#pragma unroll 8
+        for (uint32_t e = 0; e < j; ++e) {
+            first = first && bias_id[e] != id;
+        }
+        if (first) {
+            float x = widen(task.to[in]);
+#pragma unroll 8
+            for (uint32_t e = j; e < task.bias_len; ++e) {
+                x = bias_id[e] == id ? __fadd_rn(x, bias_val[e]) : x;
+            }
+            if (history && (direct ? counted(place) != 0u : (seen[place / 32u] >> place % 32u & 1u) != 0u)) {
+                uint32_t count = 0;
+                if (direct) {
+                    count = counted(place);
+                } else if (task.frequency != 0.0f) {
+                    const uint32_t at = before[place / 32u] + (uint32_t)__popc(seen[place / 32u] & ((1u << place % 32u) - 1u));
+                    if (at < WINDOW) {
+                        count = count_of[at];
+                    } else {  // (a later window's: counted by itself)
+                        for (uint32_t i = 0; i < task.history; ++i) {
+                            count += __ldg(ids.ids + i) == id ? 1u : 0u;
                         }
                     }
                 }
+                x = penalised(x, count);
+            } else if (from_slot) {
+                const uint32_t count = __ldg(slot_counts + in);
+                x = count > 0u ? penalised(x, count) : x;
+            }
+            narrow(task.to + in, x);
+        }
+    }
+    if (task.bias_len > 0u) {
+        __syncthreads();
+        for (uint32_t j = t; j < task.bias_len; j += NT) {
+            const uint32_t place = bias_id[j] - task.id0 + shift;
+            if (bias_id[j] - task.id0 < task.n) {
+                atomicAnd(kept + place / 32u, ~(1u << place % 32u));
+            }
+        }
+        __syncthreads();
+    }
+    // Values are read from `to`: the pass has just written them, they are in L2.
+    constexpr uint32_t AHEAD = 8u;
+    const uint32_t room = direct ? 4u * WINDOW : WINDOW;
+    for (uint32_t base = 0; base < total; base += room) {
+        if (base != 0u) {
+            __syncthreads();
+            if (t == 0u) {
+                next_part = 0u;
+            }
+            fill(base, t, NT, BAR_ALL);
+            __syncthreads();
+        }
+        const uint32_t held = min(room, total - base);
+        for (uint32_t e = t; e < held; e += NT * AHEAD) {
+            uint32_t place[AHEAD];
+            float x[AHEAD];
+#pragma unroll
+            for (uint32_t k = 0; k < AHEAD; ++k) {
+                place[k] = e + k * NT >= held ? NONE : !direct ? place_of[e + k * NT] : counted(e + k * NT) != 0u ? e + k * NT : NONE;
+                if (place[k] != NONE && task.keeps() && !(kept[place[k] / 32u] >> place[k] % 32u & 1u)) {
+                    place[k] = NONE;
+                }
+                if (place[k] != NONE) {
+                    x[k] = widen(task.to[place[k] - shift]);
+                }
             }
 #pragma unroll
             for (uint32_t k = 0; k < AHEAD; ++k) {
-                const uint32_t c = c0 + k * NT;
-                if (said[k] == 0u) {
-                    continue;
+                if (place[k] != NONE) {
+                    narrow(task.to + place[k] - shift, penalised(x[k], counted(e + k * NT)));
                 }
-                const uint32_t s = said[k] & 0xFFu, b = said[k] >> 8 & 0xFFu, w = said[k] >> 16 & 0xFFu;
-                float f[8];
-                unpack(raw[k], f);
-                for (uint32_t left = (s | b) & w; left != 0u; left &= left - 1u) {
-                    const uint32_t i = __ffs(left) - 1u;
-                    float x = 0.0f;
-#pragma unroll
-                    for (uint32_t j = 0; j < 8u; ++j) {
-                        x = i == j ? f[j] : x;
-                    }
-                    x = adjusted(a, m, r, c * 8u + i, x, s >> i & 1u, b >> i & 1u);
-#pragma unroll
-                    for (uint32_t j = 0; j < 8u; ++j) {
-                        f[j] = i == j ? x : f[j];
-                    }
-                }
-#pragma unroll
-                for (uint32_t i = 0; i < 8u; ++i) {
-                    f[i] = w >> i & 1u ? f[i] : neg_inf();
-                }
-                store8(to + c * 8u, f);
             }
         }
     }
-    // One logit a thread, a warp per word of marks: rows that start anywhere, and a wide row's last
-    // few logits.
-    constexpr uint32_t AHEAD = 6u;
-    const uint32_t begin = WIDE ? n / 8u * 8u : 0u;
-    for (uint32_t i0 = begin / 32u * 32u + t; i0 < n; i0 += NT * AHEAD) {
-        float f[AHEAD];
-        bool seen1[AHEAD], biased1[AHEAD], allowed1[AHEAD], any[AHEAD];
-#pragma unroll
-        for (uint32_t k = 0; k < AHEAD; ++k) {
-            const uint32_t i = i0 + k * NT;
-            any[k] = false;
-            if (i < n && i >= begin) {
-                uint32_t s, b, w;
-                words_of(m, r, i / 32u, min(32u, n - i / 32u * 32u), s, b, w);
-                seen1[k] = s >> (i % 32u) & 1u, biased1[k] = b >> (i % 32u) & 1u, allowed1[k] = w >> (i % 32u) & 1u;
-                any[k] = !(a.in_place && allowed1[k] && !seen1[k] && !biased1[k]);
-                if (any[k] && allowed1[k]) {
-                    f[k] = widen(from[i]);
-                }
-            }
-        }
-#pragma unroll
-        for (uint32_t k = 0; k < AHEAD; ++k) {
-            const uint32_t i = i0 + k * NT;
-            if (any[k]) {
-                if (!allowed1[k]) {
-                    f[k] = neg_inf();
-                } else if (seen1[k] || biased1[k]) {
-                    f[k] = adjusted(a, m, r, i, f[k], seen1[k], biased1[k]);
-                }
-                narrow(to + i, f[k]);
+    // A histogram slot's ids: its bits and counts are as they are.
+    for (uint32_t u = t; from_slot && u < units; u += NT) {
+        const int32_t first = (int32_t)(u * 32u) - (int32_t)shift;
+        uint32_t m = bits_at(slot_seen, (int32_t)task.lo + first, min(32u, (uint32_t)((int32_t)task.n - first)));
+        m &= first < 0 ? FULL << -first : FULL;  // (of the slice alone)
+        m &= first + 32 > (int32_t)task.n ? FULL >> (first + 32 - (int32_t)task.n) : FULL;
+        for (m &= task.keeps() ? kept[u] : FULL; m != 0u; m &= m - 1u) {
+            const int32_t in = first + __ffs(m) - 1;
+            const uint32_t count = __ldg(slot_counts + in);
+            if (count > 0u) {
+                narrow(task.to + in, penalised(widen(task.to[in]), count));
             }
         }
     }
 }
 
-template <typename TI, typename TO, bool WIDE, uint32_t MAX_ROWS>
-cudaError_t launch_adjust(const AdjustLaunch<MAX_ROWS> &l, uint32_t slices, uint32_t rows, size_t smem, cudaStream_t stream) {
-    auto kernel = adjust_logits_kernel<TI, TO, WIDE, MAX_ROWS>;
-    if (smem > 48u * 1024u) {
-        static std::atomic<uint64_t> ready{0};  // (bit d: device d knows)
-        int device = 0;
-        cudaError_t e = cudaGetDevice(&device);
-        const uint64_t bit = 1ull << (device & 63);
-        if (e == cudaSuccess && !(ready.load(std::memory_order_relaxed) & bit)) {
-            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)MOST_SMEM);
-            ready.fetch_or(e == cudaSuccess ? bit : 0u, std::memory_order_relaxed);
-        }
-        if (e != cudaSuccess) {
-            return e;
-        }
-    }
+constexpr uint32_t LEAST_SLICE = 2048;
+
+// How a call is cut: slices of a row, shared memory of their blocks.
+struct Cut {
+    uint32_t slices;
+    size_t smem;
+};
+
+// Shared memory of an adjusting block beside its window and bias entries: two on an SM.
+constexpr uint32_t MOST_SMEM = 66u * 1024u;
+
+template <typename Kernel, typename Launch>
+cudaError_t launch(Kernel kernel, const Launch &l, uint32_t blocks, uint32_t threads, size_t smem, cudaStream_t stream) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(slices, rows, 1);
-    cfg.blockDim = dim3(NT, 1, 1);
+    cfg.gridDim = dim3(blocks, 1, 1);
+    cfg.blockDim = dim3(threads, 1, 1);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -436,29 +666,32 @@ cudaError_t launch_adjust(const AdjustLaunch<MAX_ROWS> &l, uint32_t slices, uint
     return cudaLaunchKernelEx(&cfg, kernel, l);
 }
 
-template <uint32_t MAX_ROWS>
-cudaError_t adjust_by_type(const AdjustLaunch<MAX_ROWS> &l, uint32_t in, uint32_t out, bool wide, uint32_t slices,
-                           uint32_t rows, size_t smem, cudaStream_t stream) {
-    using B = __nv_bfloat16;
-    if (in == LILY_F32) {
-        return wide ? launch_adjust<float, float, true>(l, slices, rows, smem, stream)
-                    : launch_adjust<float, float, false>(l, slices, rows, smem, stream);
+template <typename TI, typename TO, bool WIDE, uint32_t MAX_ROWS>
+cudaError_t launch_adjust(const AdjustLaunch<MAX_ROWS> &l, const Cut &cut, cudaStream_t stream) {
+    auto kernel = adjust_logits_kernel<TI, TO, WIDE, MAX_ROWS>;
+    static std::atomic<uint64_t> ready{0};  // (bit d: device d has seen the set-up)
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    const uint64_t bit = 1ull << (device & 63);
+    if (e == cudaSuccess && !(ready.load(std::memory_order_relaxed) & bit)) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)MOST_SMEM);
+        ready.fetch_or(e == cudaSuccess ? bit : 0u, std::memory_order_relaxed);
     }
-    if (out == LILY_F32) {
-        return wide ? launch_adjust<B, float, true>(l, slices, rows, smem, stream)
-                    : launch_adjust<B, float, false>(l, slices, rows, smem, stream);
-    }
-    return wide ? launch_adjust<B, B, true>(l, slices, rows, smem, stream)
-                : launch_adjust<B, B, false>(l, slices, rows, smem, stream);
+    return e != cudaSuccess ? e : launch(kernel, l, l.a.tasks, NT, cut.smem, stream);
+}
+
+template <typename TI, typename TO, uint32_t MAX_ROWS>
+cudaError_t adjust_by_cut(const AdjustLaunch<MAX_ROWS> &l, bool wide, const Cut &cut, cudaStream_t stream) {
+    return wide ? launch_adjust<TI, TO, true, MAX_ROWS>(l, cut, stream) : launch_adjust<TI, TO, false, MAX_ROWS>(l, cut, stream);
 }
 
 // The rows [row0, row0 + rows) of a call, their penalties and slots in the launch's arguments.
 template <uint32_t MAX_ROWS>
 cudaError_t adjust_rows(const AdjustArgs &a, const lily_adjust_args_t &g, uint32_t row0, uint32_t rows, bool wide,
-                        uint32_t slices, size_t smem, cudaStream_t stream) {
+                        const Cut &cut, cudaStream_t stream) {
     AdjustLaunch<MAX_ROWS> l;
     l.a = a;
-    l.a.row0 = row0;
+    l.a.row0 = row0, l.a.rows = rows, l.a.tasks = rows * cut.slices;
     if (MAX_ROWS > 1u) {
         for (uint32_t i = 0; i < rows && i < MAX_ROWS; ++i) {
             RowPenalty &p = l.rows[i];
@@ -469,7 +702,24 @@ cudaError_t adjust_rows(const AdjustArgs &a, const lily_adjust_args_t &g, uint32
             }
         }
     }
-    return adjust_by_type(l, g.logits_dtype, g.out_dtype, wide, slices, rows, smem, stream);
+    using B = __nv_bfloat16;
+    return g.logits_dtype == LILY_F32 ? adjust_by_cut<float, float>(l, wide, cut, stream)
+           : g.out_dtype == LILY_F32  ? adjust_by_cut<B, float>(l, wide, cut, stream)
+                                      : adjust_by_cut<B, B>(l, wide, cut, stream);
+}
+
+cudaError_t mask_rows(const AdjustArgs &a, const lily_adjust_args_t &g, uint32_t row0, uint32_t rows, bool wide, const Cut &cut,
+                      cudaStream_t stream) {
+    AdjustLaunch<1> l;
+    l.a = a;
+    l.a.row0 = row0, l.a.rows = rows, l.a.tasks = rows * cut.slices;
+    using B = __nv_bfloat16;
+    const auto go = [&](auto narrow_kernel, auto wide_kernel) {
+        return launch(wide ? wide_kernel : narrow_kernel, l, l.a.tasks, MASK_NT, cut.smem, stream);
+    };
+    return g.logits_dtype == LILY_F32 ? go(mask_logits_kernel<float, float, false>, mask_logits_kernel<float, float, true>)
+           : g.out_dtype == LILY_F32  ? go(mask_logits_kernel<B, float, false>, mask_logits_kernel<B, float, true>)
+                                      : go(mask_logits_kernel<B, B, false>, mask_logits_kernel<B, B, true>);
 }
 
 constexpr uint32_t ROWS_FEW = 16, ROWS_MANY = 256;
@@ -511,13 +761,16 @@ extern "C" int32_t lily_adjust_logits(lily_sampler_t *h, void *stream_, const li
                               (g.mask_rows == nullptr && g.masks < g.rows))) {
         return fail(h, LILY_ERR_ARG, "masks of at least first_id + vocab bits, one per row if mask_rows is NULL");
     }
+    if (g.mask != nullptr && (uint64_t)g.first_id + h->vocab > 0x7FFFFFFFull) {
+        return fail(h, LILY_ERR_CAPACITY, "masks take ids up to 2^31 - 1");
+    }
     if (g.mask == nullptr && g.mask_rows != nullptr) {
         return fail(h, LILY_ERR_ARG, "mask_rows without mask");
     }
     if (g.count_slots != nullptr && (h->counts_table == nullptr || g.first_id != 0u)) {
         return fail(h, LILY_ERR_ARG, "count_slots needs LILY_FLAG_COUNTS_TABLE and first_id 0");
     }
-    bool counts = g.params != nullptr && g.params_on_device, penalties = counts;
+    bool penalties = g.params != nullptr && g.params_on_device;
     for (uint32_t r = 0; r < g.rows; ++r) {
         if (g.params != nullptr && !g.params_on_device) {
             if (!params_ok(g.params[r])) {
@@ -525,8 +778,7 @@ extern "C" int32_t lily_adjust_logits(lily_sampler_t *h, void *stream_, const li
                 std::snprintf(buf, sizeof buf, "row %u: invalid sampling parameters", r);
                 return fail(h, LILY_ERR_PARAMS, buf);
             }
-            counts = counts || g.params[r].frequency_penalty != 0.0f;
-            penalties = penalties || counts || g.params[r].presence_penalty != 0.0f || g.params[r].repetition_penalty != 1.0f;
+            penalties = penalties || g.params[r].frequency_penalty != 0.0f || g.params[r].presence_penalty != 0.0f || g.params[r].repetition_penalty != 1.0f;
         }
         if (g.count_slots != nullptr && g.count_slots[r] >= h->max_rows) {
             return fail(h, LILY_ERR_ARG, "no such histogram slot");
@@ -546,36 +798,45 @@ extern "C" int32_t lily_adjust_logits(lily_sampler_t *h, void *stream_, const li
     a.out_status = g.out_status, a.status_word = h->status_word;
     a.vocab = h->vocab, a.first_id = g.first_id, a.max_history = h->max_history, a.max_list = h->max_list;
     a.in_place = in_place ? 1u : 0u;
-    a.wide_counts = std::min<uint64_t>(g.history_ld, h->max_history) > 65535u ? 1u : 0u;
 
-    // Slices: enough blocks to fill the device, of shared memory that leaves room for two on an SM.
-    counts = counts && history;
-    const uint32_t per_id8 = 3u + (counts ? (a.wide_counts ? 32u : 16u) : 0u);  // bits of shared memory an id
-    const uint32_t most = (MOST_SMEM * 8u / per_id8) & ~255u;
-    const uint32_t want = std::max(1u, (2u * (uint32_t)h->sm_count + g.rows - 1u) / g.rows);
-    const uint32_t least = 4096u;
-    uint32_t slice = std::min(most, std::max(least, (h->vocab + want - 1u) / want));
-    slice = (slice + 255u) & ~255u;
-    uint32_t slices = (h->vocab + slice - 1u) / slice;
-    a.slice_len = slice;
-    const bool lists = history || g.bias_ids != nullptr || g.ban_ids != nullptr;
-    const size_t smem = lists ? (size_t)slice * per_id8 / 8u : 0u;
-
-    const auto rows16 = [&](const void *p, uint64_t ld, uint32_t size) {
-        return reinterpret_cast<uintptr_t>(p) % 16u == 0u && (g.rows == 1u || ld * size % 16u == 0u);
+    // Rows of both buffers miss the boundaries of eight logits alike (or not at all).
+    const bool wide = reinterpret_cast<uintptr_t>(g.logits) / in_size % 8u == reinterpret_cast<uintptr_t>(g.out) / out_size % 8u &&
+                      (g.rows == 1u || g.logits_ld % 8u == g.out_ld % 8u);
+    const bool lists = history || g.bias_ids != nullptr || (penalties && g.count_slots != nullptr);
+    const bool keeps = g.mask != nullptr || g.ban_ids != nullptr || g.bias_ids != nullptr;
+    a.history_ids = history ? g.history_ids : nullptr;
+    const uint64_t most_times = std::min<uint64_t>(g.history_ld, h->max_history);  // that a list has an id
+    const auto slice_of = [&](uint32_t count) { return ((h->vocab + count - 1u) / count + 255u) & ~255u; };
+    const auto lay_out = [&](uint32_t slice) -> size_t {  // a block's shared memory
+        const uint32_t words = slice / 32u + 8u;
+        a.direct = slice + 8u <= 2u * WINDOW ? 1u : slice + 32u <= 4u * WINDOW && most_times <= 65535u ? 2u : 0u;
+        a.seen_at = keeps ? words : 0u;
+        a.before_at = a.seen_at + (history && !a.direct ? words : 0u);
+        return (a.before_at + (history && !a.direct ? words : 0u)) * 4u;
     };
-    const bool wide = rows16(g.logits, g.logits_ld, in_size) && rows16(g.out, g.out_ld, out_size);
+    // Slices: as many as fill the device with two blocks an SM, of LEAST_SLICE logits at least.
+    const uint32_t resident = 2u * (uint32_t)h->sm_count;
+    Cut cut = {std::max(1u, std::min(resident / g.rows, (h->vocab + LEAST_SLICE - 1u) / LEAST_SLICE)), 0u};
+    while (lay_out(slice_of(cut.slices)) > (lists ? MOST_SMEM : 47u * 1024u)) {
+        ++cut.slices;
+    }
+    a.slice_len = slice_of(cut.slices);
+    cut.slices = (h->vocab + a.slice_len - 1u) / a.slice_len;  // (rounded up, they may be fewer)
+    cut.smem = lay_out(a.slice_len);
+
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     const bool plain = (g.params == nullptr || g.params_on_device) && g.count_slots == nullptr;
-    const uint32_t step = plain ? 32768u : ROWS_MANY;  // (a grid has at most 65535 rows)
+    const uint32_t step = !lists || plain ? 0x7FFFFFFFu / cut.slices : ROWS_MANY;
     for (uint32_t r = 0; r < g.rows; r += step) {
         const uint32_t rows = std::min(step, g.rows - r);
-        if (plain) {
-            CU(h, adjust_rows<1>(a, g, r, rows, wide, slices, smem, stream));
+        if (!lists) {
+            CU(h, mask_rows(a, g, r, rows, wide, cut, stream));
+        } else if (plain) {
+            CU(h, adjust_rows<1>(a, g, r, rows, wide, cut, stream));
         } else if (rows <= ROWS_FEW) {
-            CU(h, adjust_rows<ROWS_FEW>(a, g, r, rows, wide, slices, smem, stream));
+            CU(h, adjust_rows<ROWS_FEW>(a, g, r, rows, wide, cut, stream));
         } else {
-            CU(h, adjust_rows<ROWS_MANY>(a, g, r, rows, wide, slices, smem, stream));
+            CU(h, adjust_rows<ROWS_MANY>(a, g, r, rows, wide, cut, stream));
         }
     }
     return LILY_OK;

@@ -253,6 +253,52 @@ def test_counts_beyond_sixteen_bits(cuda, lily):
     assert torch.equal(logits, want)
 
 
+@pytest.mark.parametrize("rows,vocab,history", [(300, 40_000, 16_000), (100, 30_001, 9_000), (1, 9_000, 9_000), (150, 21_000, 30_000)])
+def test_more_ids_than_a_block_counts_at_a_time(cuda, lily, rows, vocab, history):
+    """Histories of all different ids, and of a row's whole vocabulary."""
+    rng = np.random.default_rng([rows, vocab])
+    case = Case(rng, rows, vocab, True, history, 12, 2)
+    for r in range(rows):  # (uniform: nearly all of them different)
+        case.history[r] = rng.integers(0, vocab, history)
+    case.history[0, :min(vocab, history)] = rng.permutation(vocab)[:history]
+    case.bias[:, 0] = case.history[:, history // 2]
+    case.bias_len[:] = 12
+    scratch = lily.SamplerScratch(vocab, max_rows=rows, max_history=history, max_list=12)
+    for out_f32, in_place in ((True, False), (False, True)):
+        _check(case, _run(cuda, lily, scratch, case, out_f32, in_place), not out_f32)
+
+
+def test_histogram_slots_with_masks_and_biases(cuda, lily):
+    torch = cuda
+    rng = np.random.default_rng(14)
+    rows, vocab = 4, 30_007
+    case = Case(rng, rows, vocab, False, 0, 20, 2)
+    counts = (rng.random((rows, vocab)) < 0.3) * rng.integers(1, 70_000, (rows, vocab))
+    case.bias[:, 1] = np.argmax(counts > 0, axis=1)
+    scratch = lily.SamplerScratch(vocab, max_rows=rows, max_list=20, counts_table=True)
+    for s in range(rows):
+        scratch.write_counts(counts[s].astype(np.uint32), slot=s)
+    kw, _ = case.args(torch, lily)
+    params = [lily.SamplingParams(repetition_penalty=1.25, frequency_penalty=0.5, presence_penalty=0.125)] * rows
+    x = case.logits.copy()
+    for r in range(rows):
+        for i, v in zip(case.bias[r, :case.bias_len[r]], case.bias_vals[r]):
+            if i < vocab:
+                x[r, i] = x[r, i] + v
+    c = counts.astype(np.float32)
+    want = np.where(counts > 0, np.where(x > 0, x / np.float32(1.25), x * np.float32(1.25)) - (np.float32(0.125) + np.float32(0.5) * c), x)
+    for r in range(rows):
+        want[r, [i for i in case.ban[r, :case.ban_len[r]] if i < vocab]] = -np.inf
+        if case.mask_rows[r] >= 0:
+            want[r, ~case.bits[case.mask_rows[r], :vocab]] = -np.inf
+    for in_place in (False, True):
+        logits = torch.from_numpy(case.logits).cuda()
+        out = logits if in_place else torch.empty_like(logits)
+        scratch.adjust_logits(logits, params, None if in_place else out, count_slots=list(range(rows)), **kw)
+        assert np.array_equal(out.cpu().numpy().view(np.uint32), want.astype(np.float32).view(np.uint32))
+    assert scratch.status() == 0
+
+
 def test_histogram_slots(cuda, lily):
     torch = cuda
     rng = np.random.default_rng(4)
