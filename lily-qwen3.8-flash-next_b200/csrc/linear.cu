@@ -11,6 +11,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cstring>
+#include <type_traits>
 
 #include "../../include/lily_layers.h"
 #include "handle.cuh"
@@ -43,29 +44,30 @@ struct LinearArgs {
     uint32_t lost_stage;    // test hook: the first block leaves out the copies of this step (~0: none)
 };
 
-// Sixteen values through the activation. One branch for all of them: with the branch inside, sixteen
+// C values through the activation. One branch for all of them: with the branch inside, sixteen
 // copies of every function's code lay in the epilogue's loop, which then ran from instruction misses
 // (4099 x 4096 x 4096 without an activation 120 us, with a residual 331).
-__device__ __forceinline__ void activate(float (&v)[16], uint32_t activation) {
+template <uint32_t C>
+__device__ __forceinline__ void activate(float (&v)[C], uint32_t activation) {
     if (activation == LILY_ACT_NONE) {
     } else if (activation == LILY_ACT_RELU) {
 #pragma unroll
-        for (uint32_t j = 0; j < 16u; ++j) {
+        for (uint32_t j = 0; j < C; ++j) {
             v[j] = v[j] < 0.0f ? 0.0f : v[j];  // (a NaN stays)
         }
     } else if (activation == LILY_ACT_SILU) {
 #pragma unroll
-        for (uint32_t j = 0; j < 16u; ++j) {
+        for (uint32_t j = 0; j < C; ++j) {
             v[j] = __fdividef(v[j], 1.0f + expf(-v[j]));
         }
     } else if (activation == LILY_ACT_GELU) {
 #pragma unroll
-        for (uint32_t j = 0; j < 16u; ++j) {
+        for (uint32_t j = 0; j < C; ++j) {
             v[j] = 0.5f * v[j] * (1.0f + erff(v[j] * 0.70710678f));
         }
     } else {
 #pragma unroll
-        for (uint32_t j = 0; j < 16u; ++j) {
+        for (uint32_t j = 0; j < C; ++j) {
             const float u = 0.79788456f * (v[j] + 0.044715f * v[j] * v[j] * v[j]);
             v[j] = __fdividef(v[j], 1.0f + expf(-2.0f * u));  // (1 + tanh(u)) / 2 = 1 / (1 + exp(-2 u))
         }
@@ -90,55 +92,57 @@ __device__ __forceinline__ Output output_of(const LinearArgs &a, uint32_t n) {
     return o;
 }
 
-// The residuals of output n and of up to sixteen tokens from t on.
+// The residuals of output n and of up to C tokens from t on.
+template <uint32_t C>
 __device__ __forceinline__ void residuals_of(const LinearArgs &a, const Output &o, uint32_t t, uint32_t n, uint32_t live,
-                                             float (&r)[16]) {
+                                             float (&r)[C]) {
     if (a.residual == nullptr || !o.live) {
 #pragma unroll
-        for (uint32_t j = 0; j < 16u; ++j) {
+        for (uint32_t j = 0; j < C; ++j) {
             r[j] = 0.0f;
         }
     } else if (a.out_f32) {
         const float *p = static_cast<const float *>(a.residual) + (uint64_t)t * a.residual_ld + n;
 #pragma unroll
-        for (uint32_t j = 0; j < 16u; ++j) {
+        for (uint32_t j = 0; j < C; ++j) {
             r[j] = j < live ? p[j * a.residual_ld] : 0.0f;
         }
     } else {
         const __nv_bfloat16 *p = static_cast<const __nv_bfloat16 *>(a.residual) + (uint64_t)t * a.residual_ld + n;
 #pragma unroll
-        for (uint32_t j = 0; j < 16u; ++j) {
+        for (uint32_t j = 0; j < C; ++j) {
             r[j] = j < live ? __bfloat162float(p[j * a.residual_ld]) : 0.0f;
         }
     }
 }
 
-// The sums v of output n and of up to sixteen tokens from t on, finished and written. (A whole warp:
+// The sums v of output n and of up to C tokens from t on, finished and written. (A whole warp:
 // lane j has token j's scale.)
-__device__ __forceinline__ void finish(const LinearArgs &a, const Output &o, uint32_t t, uint32_t n, uint32_t live, float (&v)[16],
-                                       const float (&r)[16]) {
+template <uint32_t C>
+__device__ __forceinline__ void finish(const LinearArgs &a, const Output &o, uint32_t t, uint32_t n, uint32_t live, float (&v)[C],
+                                       const float (&r)[C]) {
     if (a.a_scales != nullptr) {
         const uint32_t lane = threadIdx.x % 32u;
-        const float mine = lane < min(live, 16u) ? __ldg(a.a_scales + t + lane) : 0.0f;
+        const float mine = lane < min(live, C) ? __ldg(a.a_scales + t + lane) : 0.0f;
 #pragma unroll
-        for (uint32_t j = 0; j < 16u; ++j) {
+        for (uint32_t j = 0; j < C; ++j) {
             v[j] *= __shfl_sync(FULL, mine, j) * o.scale;
         }
     }
 #pragma unroll
-    for (uint32_t j = 0; j < 16u; ++j) {
+    for (uint32_t j = 0; j < C; ++j) {
         v[j] += o.bias;
     }
     activate(v, a.activation);
 #pragma unroll
-    for (uint32_t j = 0; j < 16u; ++j) {
+    for (uint32_t j = 0; j < C; ++j) {
         v[j] += r[j];
     }
     if (!o.live) {
     } else if (a.out_f32) {
         float *p = static_cast<float *>(a.out) + (uint64_t)t * a.out_ld + n;
 #pragma unroll
-        for (uint32_t j = 0; j < 16u; ++j) {
+        for (uint32_t j = 0; j < C; ++j) {
             if (j < live) {
                 p[j * a.out_ld] = v[j];
             }
@@ -146,7 +150,7 @@ __device__ __forceinline__ void finish(const LinearArgs &a, const Output &o, uin
     } else {
         __nv_bfloat16 *p = static_cast<__nv_bfloat16 *>(a.out) + (uint64_t)t * a.out_ld + n;
 #pragma unroll
-        for (uint32_t j = 0; j < 16u; ++j) {
+        for (uint32_t j = 0; j < C; ++j) {
             if (j < live) {
                 p[j * a.out_ld] = __float2bfloat16_rn(v[j]);
             }
@@ -182,6 +186,12 @@ __device__ __forceinline__ void mma_ss(uint32_t d_tmem, uint64_t adesc, uint64_t
 
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ uint32_t at_rank(uint32_t addr, uint32_t rank) {
+    uint32_t there;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(addr), "r"(rank));
+    return there;
+}
 
 // ------------------------------------------------------------------ few tokens --
 //
@@ -314,37 +324,63 @@ __global__ void __launch_bounds__(192) linear_few_kernel(const __grid_constant__
     const uint32_t accs = min(S::ACCS, steps), from = tmem + (quad * 32u << 16);
     // Sixteen tokens' sums of this thread's output.
     const auto sums_of = [&](uint32_t c, float (&v)[16]) {
-        uint32_t q[16];
-        tmem_ld16(from + c, q);
+        uint32_t q[S::ACCS][16];
+#pragma unroll
+        for (uint32_t k = 0; k < S::ACCS; ++k) {
+            if (k < accs) {
+                tmem_ld16(from + k * N + c, q[k]);
+            }
+        }
         tmem_ld_wait();
 #pragma unroll
         for (uint32_t j = 0; j < 16u; ++j) {
-            v[j] = __uint_as_float(q[j]);
+            v[j] = __uint_as_float(q[0][j]);
         }
-        for (uint32_t k = 1; k < accs; ++k) {
-            tmem_ld16(from + k * N + c, q);
-            tmem_ld_wait();
 #pragma unroll
-            for (uint32_t j = 0; j < 16u; ++j) {
-                v[j] += __uint_as_float(q[j]);
+        for (uint32_t k = 1; k < S::ACCS; ++k) {
+            if (k < accs) {
+#pragma unroll
+                for (uint32_t j = 0; j < 16u; ++j) {
+                    v[j] += __uint_as_float(q[k][j]);
+                }
             }
         }
     };
     if (shares == 1u) {
         if (warp >= 2u) {
             const Output o = output_of(a, n);
+            float r[16];
+            residuals_of(a, o, token0, n, live, r);  // (asked for a round ahead, here and below)
             warp_wait(base + S::FINAL, 0u, abort_word, a.wait_ns);
             tc_fence_after();
             for (uint32_t c = 0; c < live; c += 16u) {
-                float v[16], r[16];
-                residuals_of(a, o, token0 + c, n, live - c, r);
+                float v[16], next[16];
+                residuals_of(a, o, token0 + c + 16u, n, live > c + 16u ? live - c - 16u : 0u, next);
                 sums_of(c, v);
                 finish(a, o, token0 + c, n, live - c, v, r);
+#pragma unroll
+                for (uint32_t j = 0; j < 16u; ++j) {
+                    r[j] = next[j];
+                }
             }
         }
     } else {
-        // Token c is finished by block c / per; its sums lie there at [share][c % per][output].
-        const uint32_t per = N / shares;
+        // Token c is finished by block c / per; its sums lie there at [share][output][c % per], four tokens
+        // (or both) side by side, which an output's thread sends and takes together. (One by one the
+        // sums of 128 tokens took 3.6 us to send and 13 to add up.)
+        const uint32_t per = N / shares, log_per = 31u - __clz(per);  // (powers of two)
+        const uint32_t first = rank * per, mine = first < live ? min(per, live - first) : 0u;
+        const uint32_t quads = per / 4u;
+        const auto part_at = [&](uint32_t share, uint32_t c) {  // (neighbours' quads lie in different banks)
+            return base + S::PART + (share * TILE_M + row) * per * 4u + (((c / 4u) ^ (row & (quads - 1u))) * 16u);
+        };
+        // What does not depend on the sums is asked for before they are there.
+        Output o = {1.0f, 0.0f, false};
+        float r[16];
+        if (warp >= 2u) {
+            o = output_of(a, n);
+            residuals_of(a, o, token0 + first, n, mine, r);
+        }
         cluster_wait();
         if (warp >= 2u) {
             warp_wait(base + S::FINAL, 0u, abort_word, a.wait_ns);
@@ -352,13 +388,23 @@ __global__ void __launch_bounds__(192) linear_few_kernel(const __grid_constant__
             for (uint32_t c = 0; c < live; c += 16u) {
                 float v[16];
                 sums_of(c, v);
+                if (per == 2u) {
 #pragma unroll
-                for (uint32_t j = 0; j < 16u; ++j) {
-                    if (c + j < live) {
-                        const uint32_t here = base + S::PART + ((rank * per + (c + j) % per) * TILE_M + row) * 4u;
-                        uint32_t there;
-                        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(here), "r"((c + j) / per));
-                        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(there), "f"(v[j]) : "memory");
+                    for (uint32_t j = 0; j < 16u; j += 2u) {
+                        if (c + j < live) {
+                            const uint32_t there = at_rank(base + S::PART + (rank * TILE_M + row) * 8u, (c + j) / 2u);
+                            asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(there), "f"(v[j]), "f"(v[j + 1u]) : "memory");
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (uint32_t j = 0; j < 16u; j += 4u) {
+                        if (c + j < live) {
+                            const uint32_t there = at_rank(part_at(rank, (c + j) & (per - 1u)), (c + j) >> log_per);
+                            asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(there), "f"(v[j]), "f"(v[j + 1u]),
+                                         "f"(v[j + 2u]), "f"(v[j + 3u])
+                                         : "memory");
+                        }
                     }
                 }
             }
@@ -367,22 +413,47 @@ __global__ void __launch_bounds__(192) linear_few_kernel(const __grid_constant__
         cluster_arrive();
         cluster_wait();
         if (warp >= 2u) {
-            const Output o = output_of(a, n);
-            const float *part = reinterpret_cast<const float *>(smem + S::PART) + row;
-            const uint32_t first = rank * per, mine = first < live ? min(per, live - first) : 0u;
-            for (uint32_t c = 0; c < mine; c += 16u) {
-                float v[16], r[16];
-                residuals_of(a, o, token0 + first + c, n, mine - c, r);
+            if (per == 2u) {
+                float v[2] = {0.0f, 0.0f}, r2[2] = {r[0], r[1]};
+                const float2 *part = reinterpret_cast<const float2 *>(smem + S::PART) + row;
 #pragma unroll
-                for (uint32_t j = 0; j < 16u; ++j) {
-                    v[j] = 0.0f;
-                    if (c + j < mine) {
-                        for (uint32_t k = 0; k < shares; ++k) {
-                            v[j] += part[(k * per + c + j) * TILE_M];
-                        }
-                    }
+                for (uint32_t k = 0; k < 8u; ++k) {  // (two tokens a block: eight blocks)
+                    const float2 p = part[k * TILE_M];
+                    v[0] += p.x, v[1] += p.y;
                 }
-                finish(a, o, token0 + first + c, n, mine - c, v, r);
+                if (mine > 0u) {
+                    finish(a, o, token0 + first, n, mine, v, r2);
+                }
+            } else {
+                const auto finish_all = [&](auto at_once) {
+                    constexpr uint32_t C = decltype(at_once)::value;
+                    for (uint32_t c = 0; c < mine; c += C) {
+                        float v[C] = {}, rc[C];
+                        if (c == 0u) {
+#pragma unroll
+                            for (uint32_t j = 0; j < C; ++j) {
+                                rc[j] = r[j];
+                            }
+                        } else {
+                            residuals_of(a, o, token0 + first + c, n, mine - c, rc);
+                        }
+                        for (uint32_t k = 0; k < shares; ++k) {
+#pragma unroll
+                            for (uint32_t j = 0; j < C; j += 4u) {
+                                const float4 p = *reinterpret_cast<const float4 *>(smem + (part_at(k, c + j) - base));
+                                v[j] += p.x, v[j + 1u] += p.y, v[j + 2u] += p.z, v[j + 3u] += p.w;
+                            }
+                        }
+                        finish(a, o, token0 + first + c, n, mine - c, v, rc);
+                    }
+                };
+                if (per == 4u) {  // (no code for tokens that are not there: most of it runs once, and waits for itself)
+                    finish_all(std::integral_constant<uint32_t, 4>());
+                } else if (per == 8u) {
+                    finish_all(std::integral_constant<uint32_t, 8>());
+                } else {
+                    finish_all(std::integral_constant<uint32_t, 16>());
+                }
             }
         }
     }
@@ -427,12 +498,6 @@ struct Many {
     static constexpr uint32_t BYTES = ABORT + 4u + 1024u;
     static_assert(BYTES <= 227u * 1024u, "shared memory of one block");
 };
-
-__device__ __forceinline__ uint32_t at_rank(uint32_t addr, uint32_t rank) {
-    uint32_t there;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(addr), "r"(rank));
-    return there;
-}
 
 // A copy into this block's shared memory whose bytes complete a barrier of either block of the pair.
 __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap *map, uint32_t cluster_bar, int32_t x, int32_t y) {
