@@ -195,9 +195,10 @@ __device__ __forceinline__ uint32_t at_rank(uint32_t addr, uint32_t rank) {
 
 // ------------------------------------------------------------------ few tokens --
 //
-// One tile of 128 outputs x N tokens per cluster; the cluster's blocks share the columns out
-// evenly. Each sums its share in tensor memory, then sends every token's column of sums to the
-// block that finishes that token, which adds the shares up in the blocks' order.
+// Tiles of 128 outputs x N tokens. Many of them: a block has one after the other, and finishes one while
+// it multiplies the next. Few: a cluster has one, whose columns its blocks share out evenly. Each
+// sums its share in tensor memory, then sends every token's column of sums to the block that finishes that
+// token, which adds the shares up in the blocks' order.
 //
 // A block's warps: 0 asks for the copies, 1 issues the multiplies, 2 to 5 are the epilogue.
 template <uint32_t N>
@@ -207,19 +208,26 @@ struct Few {
     static constexpr uint32_t STAGE = A_STAGE + B_STAGE;
     static constexpr uint32_t PART_BYTES = N * TILE_M * 4u;
     // Two blocks on an SM up to 64 tokens, else one.
-    static constexpr uint32_t STAGES = N == 16u ? 5u : N == 32u ? 4u : N == 64u ? 3u : 4u;
-    // Sums of successive steps go into accumulators in turn: shorter chains of additions.
-    static constexpr uint32_t ACCS = N <= 64u ? 4u : 2u;
-    static constexpr uint32_t COLS = ACCS * N < 32u ? 32u : ACCS * N;
-    static constexpr uint32_t PART = STAGES * STAGE;
-    static constexpr uint32_t BARS = PART + PART_BYTES;
+    static constexpr uint32_t STAGES = N == 16u ? 5u : N == 32u ? 4u : N == 64u ? 4u : 6u;
+    // The sums that blocks send one another have a place of their own (a block may send as soon as the
+    // other runs), or, where that takes a stage, the stages' (it has to be done with its columns).
+    static constexpr bool OVER_STAGES = N >= 64u;
+    // Sums of successive steps go into accumulators in turn: shorter chains of additions. Two sets of them: a
+    // tile is finished while the block's next one is multiplied.
+    static constexpr uint32_t ACCS = N <= 64u ? 2u : 1u, SETS = 2;
+    static constexpr uint32_t COLS = SETS * ACCS * N;
+    static constexpr uint32_t PART = OVER_STAGES ? 0u : STAGES * STAGE;
+    static constexpr uint32_t BARS = STAGES * STAGE + (OVER_STAGES ? 0u : PART_BYTES);
+    static_assert(PART_BYTES <= STAGES * STAGE, "room for the sums");
     static constexpr uint32_t EMPTY = BARS + 8u * STAGES;
-    static constexpr uint32_t FINAL = EMPTY + 8u * STAGES;
+    static constexpr uint32_t ACC_FULL = EMPTY + 8u * STAGES;
+    static constexpr uint32_t ACC_EMPTY = ACC_FULL + 8u * SETS;
+    static constexpr uint32_t FINAL = ACC_EMPTY + 8u * SETS;
     static constexpr uint32_t TMEM_ADDR = FINAL + 8u;
     static constexpr uint32_t ABORT = TMEM_ADDR + 4u;
     static constexpr uint32_t BYTES = ABORT + 4u + 1024u;
     static_assert(BYTES <= 227u * 1024u && BYTES > 76u * 1024u, "at most two blocks on an SM");
-    static_assert(COLS <= 256u && (COLS & (COLS - 1u)) == 0u, "tensor memory of two blocks on an SM");
+    static_assert(COLS >= 32u && COLS <= 256u && (COLS & (COLS - 1u)) == 0u, "tensor memory of two blocks on an SM");
 };
 
 template <uint32_t N, bool E4M3>
@@ -233,8 +241,10 @@ __global__ void __launch_bounds__(192) linear_few_kernel(const __grid_constant__
     uint32_t rank, shares;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(shares));
-    const uint32_t tile = blockIdx.x / shares;
-    const uint32_t token0 = tile % a.token_tiles * N, output0 = tile / a.token_tiles * TILE_M;
+    const uint32_t tile0 = blockIdx.x / shares, stride = gridDim.x / shares;
+    const uint32_t tiles = (a.outputs + TILE_M - 1u) / TILE_M * a.token_tiles;
+    const auto token_of = [&](uint32_t tile) { return tile % a.token_tiles * N; };
+    const auto output_tile = [&](uint32_t tile) { return tile / a.token_tiles * TILE_M; };
     const uint32_t block0 = (uint32_t)((uint64_t)a.blocks * rank / shares);
     const uint32_t steps = (uint32_t)((uint64_t)a.blocks * (rank + 1u) / shares) - block0;
 
@@ -242,6 +252,10 @@ __global__ void __launch_bounds__(192) linear_few_kernel(const __grid_constant__
         for (uint32_t s = 0; s < S::STAGES; ++s) {
             mbar_init(base + S::BARS + 8 * s, 1);
             mbar_init(base + S::EMPTY + 8 * s, 1);
+        }
+        for (uint32_t b = 0; b < S::SETS; ++b) {
+            mbar_init(base + S::ACC_FULL + 8 * b, 1);
+            mbar_init(base + S::ACC_EMPTY + 8 * b, 4);
         }
         mbar_init(base + S::FINAL, 1);
         *abort_word = 0;
@@ -257,7 +271,7 @@ __global__ void __launch_bounds__(192) linear_few_kernel(const __grid_constant__
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(smem + S::TMEM_ADDR);
-    if (shares > 1u) {
+    if (shares > 1u && !S::OVER_STAGES) {
         cluster_arrive();  // (this block has begun: the others may write into its shared memory)
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -267,22 +281,26 @@ __global__ void __launch_bounds__(192) linear_few_kernel(const __grid_constant__
 
     if (warp == 0u) {
         if (lane == 0u) {
-            uint32_t asked = 0, parity = 0;
-            for (uint32_t i = 0; i < steps; ++i) {
-                const uint32_t s = i % S::STAGES, use = i / S::STAGES;
-                if (mbar_wait(base + S::EMPTY + 8 * s, (use & 1u) ^ 1u, abort_word, a.wait_ns)) {
-                    break;
+            uint32_t asked = 0, parity = 0, i = 0;
+            for (uint32_t tile = tile0; tile < tiles; tile += stride) {
+                const int32_t token0 = (int32_t)token_of(tile), output0 = (int32_t)output_tile(tile);
+                for (uint32_t k = 0; k < steps; ++k, ++i) {
+                    const uint32_t s = i % S::STAGES, use = i / S::STAGES;
+                    if (mbar_wait(base + S::EMPTY + 8 * s, (use & 1u) ^ 1u, abort_word, a.wait_ns)) {
+                        tile = tiles - stride;  // (the last one)
+                        break;
+                    }
+                    const uint32_t bar = base + S::BARS + 8 * s, to = base + s * S::STAGE;
+                    const int32_t x = (int32_t)((block0 + k) * (E4M3 ? BLOCK_BYTES : BLOCK_BYTES / 2u));
+                    if (i == a.lost_stage && blockIdx.x == 0u) {
+                        continue;  // (test hook: the stage never fills)
+                    }
+                    asked |= 1u << s;
+                    parity = (parity & ~(1u << s)) | (use & 1u) << s;
+                    mbar_expect_tx(bar, S::STAGE);
+                    tma_load_2d(to, &a.w_map, bar, x, output0);
+                    tma_load_2d(to + A_STAGE, &a.a_map, bar, x, token0);
                 }
-                const uint32_t bar = base + S::BARS + 8 * s, to = base + s * S::STAGE;
-                const int32_t x = (int32_t)((block0 + i) * (E4M3 ? BLOCK_BYTES : BLOCK_BYTES / 2u));
-                if (i == a.lost_stage && blockIdx.x == 0u) {
-                    continue;  // (test hook: the stage never fills)
-                }
-                asked |= 1u << s;
-                parity = (parity & ~(1u << s)) | (use & 1u) << s;
-                mbar_expect_tx(bar, S::STAGE);
-                tma_load_2d(to, &a.w_map, bar, x, (int32_t)output0);
-                tma_load_2d(to + A_STAGE, &a.a_map, bar, x, (int32_t)token0);
             }
             if (*abort_word) {  // the copies asked for land in this block's shared memory: it stays until they have
                 for (uint32_t s = 0; s < S::STAGES; ++s) {
@@ -296,19 +314,32 @@ __global__ void __launch_bounds__(192) linear_few_kernel(const __grid_constant__
     } else if (warp == 1u) {
         const bool leader = elect_one();
         const uint32_t idesc = product_desc<E4M3>(TILE_M, N);
-        for (uint32_t i = 0; i < steps; ++i) {
-            const uint32_t s = i % S::STAGES;
-            if (warp_wait(base + S::BARS + 8 * s, i / S::STAGES & 1u, abort_word, a.wait_ns)) {
+        uint32_t i = 0, turn = 0;
+        bool gave_up = false;
+        for (uint32_t tile = tile0; tile < tiles && !gave_up; tile += stride, ++turn) {
+            const uint32_t b = turn % S::SETS;
+            if (warp_wait(base + S::ACC_EMPTY + 8 * b, (turn / S::SETS & 1u) ^ 1u, abort_word, a.wait_ns)) {
                 break;
             }
-            tc_fence_after();
-            if (leader) {
-                const uint64_t adesc = operand_desc(base + s * S::STAGE), bdesc = operand_desc(base + s * S::STAGE + A_STAGE);
-#pragma unroll
-                for (uint32_t k = 0; k < 4u; ++k) {
-                    mma_ss<E4M3>(tmem + i % S::ACCS * N, adesc + 2u * k, bdesc + 2u * k, idesc, i >= S::ACCS || k > 0u);
+            for (uint32_t k = 0; k < steps; ++k, ++i) {
+                const uint32_t s = i % S::STAGES;
+                if (warp_wait(base + S::BARS + 8 * s, i / S::STAGES & 1u, abort_word, a.wait_ns)) {
+                    gave_up = true;
+                    break;
                 }
-                mma_commit(base + S::EMPTY + 8 * s);
+                tc_fence_after();
+                if (leader) {
+                    const uint64_t adesc = operand_desc(base + s * S::STAGE), bdesc = operand_desc(base + s * S::STAGE + A_STAGE);
+#pragma unroll
+                    for (uint32_t q = 0; q < 4u; ++q) {
+                        mma_ss<E4M3>(tmem + (b * S::ACCS + k % S::ACCS) * N, adesc + 2u * q, bdesc + 2u * q, idesc, k >= S::ACCS || q > 0u);
+                    }
+                    mma_commit(base + S::EMPTY + 8 * s);
+                }
+                __syncwarp();
+            }
+            if (leader && !gave_up) {
+                mma_commit(base + S::ACC_FULL + 8 * b);
             }
             __syncwarp();
         }
@@ -320,15 +351,14 @@ __global__ void __launch_bounds__(192) linear_few_kernel(const __grid_constant__
     }
 
     const uint32_t quad = warp % 4u, row = quad * 32u + lane;  // the epilogue's lanes of tensor memory
-    const uint32_t n = output0 + row, live = min(N, a.tokens - token0);
     const uint32_t accs = min(S::ACCS, steps), from = tmem + (quad * 32u << 16);
-    // Sixteen tokens' sums of this thread's output.
-    const auto sums_of = [&](uint32_t c, float (&v)[16]) {
+    // Sixteen tokens' sums of this thread's output, of set b.
+    const auto sums_of = [&](uint32_t b, uint32_t c, float (&v)[16]) {
         uint32_t q[S::ACCS][16];
 #pragma unroll
         for (uint32_t k = 0; k < S::ACCS; ++k) {
             if (k < accs) {
-                tmem_ld16(from + k * N + c, q[k]);
+                tmem_ld16(from + (b * S::ACCS + k) * N + c, q[k]);
             }
         }
         tmem_ld_wait();
@@ -347,16 +377,27 @@ __global__ void __launch_bounds__(192) linear_few_kernel(const __grid_constant__
         }
     };
     if (shares == 1u) {
-        if (warp >= 2u) {
+        uint32_t turn = 0;
+        for (uint32_t tile = tile0; warp >= 2u && tile < tiles; tile += stride, ++turn) {
+            const uint32_t b = turn % S::SETS, token0 = token_of(tile), n = output_tile(tile) + row, live = min(N, a.tokens - token0);
             const Output o = output_of(a, n);
             float r[16];
             residuals_of(a, o, token0, n, live, r);  // (asked for a round ahead, here and below)
-            warp_wait(base + S::FINAL, 0u, abort_word, a.wait_ns);
+            if (warp_wait(base + S::ACC_FULL + 8 * b, turn / S::SETS & 1u, abort_word, a.wait_ns)) {
+                break;
+            }
             tc_fence_after();
             for (uint32_t c = 0; c < live; c += 16u) {
                 float v[16], next[16];
                 residuals_of(a, o, token0 + c + 16u, n, live > c + 16u ? live - c - 16u : 0u, next);
-                sums_of(c, v);
+                sums_of(b, c, v);
+                if (c + 16u >= live) {  // (the sums are in registers)
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0u) {
+                        mbar_arrive(base + S::ACC_EMPTY + 8 * b);
+                    }
+                }
                 finish(a, o, token0 + c, n, live - c, v, r);
 #pragma unroll
                 for (uint32_t j = 0; j < 16u; ++j) {
@@ -368,6 +409,7 @@ __global__ void __launch_bounds__(192) linear_few_kernel(const __grid_constant__
         // Token c is finished by block c / per; its sums lie there at [share][output][c % per], four tokens
         // (or both) side by side, which an output's thread sends and takes together. (One by one the
         // sums of 128 tokens took 3.6 us to send and 13 to add up.)
+        const uint32_t token0 = token_of(tile0), n = output_tile(tile0) + row, live = min(N, a.tokens - token0);
         const uint32_t per = N / shares, log_per = 31u - __clz(per);  // (powers of two)
         const uint32_t first = rank * per, mine = first < live ? min(per, live - first) : 0u;
         const uint32_t quads = per / 4u;
@@ -381,13 +423,19 @@ __global__ void __launch_bounds__(192) linear_few_kernel(const __grid_constant__
             o = output_of(a, n);
             residuals_of(a, o, token0 + first, n, mine, r);
         }
+        if (warp >= 2u) {
+            warp_wait(base + S::ACC_FULL, 0u, abort_word, a.wait_ns);
+            tc_fence_after();
+        }
+        __syncwarp();
+        if (S::OVER_STAGES) {
+            cluster_arrive();
+        }
         cluster_wait();
         if (warp >= 2u) {
-            warp_wait(base + S::FINAL, 0u, abort_word, a.wait_ns);
-            tc_fence_after();
             for (uint32_t c = 0; c < live; c += 16u) {
                 float v[16];
-                sums_of(c, v);
+                sums_of(0u, c, v);
                 if (per == 2u) {
 #pragma unroll
                     for (uint32_t j = 0; j < 16u; j += 2u) {
@@ -713,14 +761,14 @@ cudaError_t set_up(Kernel kernel, uint32_t bytes, std::atomic<uint64_t> &ready) 
 }
 
 template <uint32_t N, bool E4M3>
-cudaError_t launch_few(const LinearArgs &a, uint32_t tiles, uint32_t shares, cudaStream_t stream) {
+cudaError_t launch_few(const LinearArgs &a, uint32_t blocks, uint32_t shares, cudaStream_t stream) {
     static std::atomic<uint64_t> ready{0};
     const cudaError_t e = set_up(linear_few_kernel<N, E4M3>, Few<N>::BYTES, ready);
     if (e != cudaSuccess) {
         return e;
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(tiles * shares, 1, 1);
+    cfg.gridDim = dim3(blocks, 1, 1);
     cfg.blockDim = dim3(Few<N>::THREADS, 1, 1);
     cfg.dynamicSmemBytes = Few<N>::BYTES;
     cfg.stream = stream;
@@ -757,11 +805,11 @@ cudaError_t launch_many(const LinearArgs &a, uint32_t pairs, cudaStream_t stream
 }
 
 template <bool E4M3>
-cudaError_t few_by_tokens(const LinearArgs &a, uint32_t n, uint32_t tiles, uint32_t shares, cudaStream_t stream) {
-    return n == 16u   ? launch_few<16, E4M3>(a, tiles, shares, stream)
-           : n == 32u ? launch_few<32, E4M3>(a, tiles, shares, stream)
-           : n == 64u ? launch_few<64, E4M3>(a, tiles, shares, stream)
-                      : launch_few<128, E4M3>(a, tiles, shares, stream);
+cudaError_t few_by_tokens(const LinearArgs &a, uint32_t n, uint32_t blocks, uint32_t shares, cudaStream_t stream) {
+    return n == 16u   ? launch_few<16, E4M3>(a, blocks, shares, stream)
+           : n == 32u ? launch_few<32, E4M3>(a, blocks, shares, stream)
+           : n == 64u ? launch_few<64, E4M3>(a, blocks, shares, stream)
+                      : launch_few<128, E4M3>(a, blocks, shares, stream);
 }
 
 bool encode_rows(CUtensorMap *map, const void *p, uint64_t ld, uint32_t rows, uint32_t columns, uint32_t dtype,
@@ -858,16 +906,18 @@ extern "C" int32_t lily_linear(lily_sampler_t *h, void *stream_, const lily_line
     }
     a.token_tiles = (g.tokens + n - 1u) / n;
     const uint64_t tiles = (uint64_t)a.token_tiles * ((g.outputs + TILE_M - 1u) / TILE_M);
-    if (tiles > 0x7FFFFFFFull / 8u) {
+    if (tiles > 0x7FFFFFFFull) {
         return fail(h, LILY_ERR_CAPACITY, "more tiles than a launch takes");
     }
-    // Shares of the columns: as many blocks as the device holds at once, of four steps at least.
-    const uint32_t room = (uint32_t)h->sm_count * (n <= 64u ? 2u : 1u);
+    // Shares of the columns: as many blocks as there are SMs, of four steps at least; up to 32 tokens two on
+    // an SM, of eight (24 x 4096 x 4096: e4m3, four shares of eight steps 7.7 us, eight of four 8.2; bf16, of
+    // sixteen 10.6, of eight 9.4; 64 tokens on one block an SM 12.7 us, on two 14.1).
+    const uint64_t sms = (uint32_t)h->sm_count;
     uint32_t shares = 8u;
-    while (shares > 1u && (tiles * shares > room || a.blocks < 4u * shares)) {
+    while (shares > 1u && (tiles * shares > sms * (n <= 32u ? 2u : 1u) || a.blocks < (tiles * shares > sms ? 8u : 4u) * shares)) {
         shares /= 2u;
     }
-    CU(h, e4m3 ? few_by_tokens<true>(a, n, (uint32_t)tiles, shares, stream)
-               : few_by_tokens<false>(a, n, (uint32_t)tiles, shares, stream));
+    const uint32_t blocks = (uint32_t)std::min<uint64_t>(tiles, sms * (n <= 64u ? 2u : 1u)) * shares;
+    CU(h, e4m3 ? few_by_tokens<true>(a, n, blocks, shares, stream) : few_by_tokens<false>(a, n, blocks, shares, stream));
     return LILY_OK;
 }
