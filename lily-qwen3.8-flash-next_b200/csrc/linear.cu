@@ -30,7 +30,8 @@ constexpr uint32_t FULL = 0xFFFFFFFFu;
 
 struct LinearArgs {
     CUtensorMap w_map;  // [outputs, columns], boxes of 128 rows x 128 bytes, 128-byte swizzle
-    CUtensorMap a_map;  // [tokens, columns], boxes of a token tile x 128 bytes
+    CUtensorMap a_map;  // [tokens, columns], boxes of a token tile (many tokens: half of one) x 128 bytes
+    CUtensorMap out_map, residual_map;  // many tokens, `copies`: bf16 [tokens, outputs], boxes of half a tile x 32 outputs
     const float *a_scales, *w_scales;
     const void *bias, *residual;
     void *out;
@@ -38,17 +39,32 @@ struct LinearArgs {
     uint32_t tokens, outputs;
     uint32_t blocks;        // steps of BLOCK_BYTES in a row
     uint32_t token_tiles;
+    uint32_t tile_tokens;   // many tokens: of a tile, a multiple of 32
+    uint32_t copies;        // many tokens: out and residual go through shared memory
     uint32_t out_f32, bias_f32, activation;
     uint32_t *status_word;
     uint64_t wait_ns;
     uint32_t lost_stage;    // test hook: the first block leaves out the copies of this step (~0: none)
 };
 
+// The normal distribution's integral up to v, (1 + erf(v / sqrt(2))) / 2, by Abramowitz and Stegun's 7.1.26: at
+// most 7.5e-8 off, a third of erff's instructions and none that a lane takes alone. For results of 8 bits.
+__device__ __forceinline__ float normal_integral(float v) {
+    const float x = fabsf(v) * 0.70710678f;
+    const float t = __fdividef(1.0f, fmaf(0.3275911f, x, 1.0f));
+    float p = fmaf(1.061405429f, t, -1.453152027f);
+    p = fmaf(p, t, 1.421413741f);
+    p = fmaf(p, t, -0.284496736f);
+    p = fmaf(p, t, 0.254829592f);
+    const float tail = 0.5f * p * t * __expf(-x * x);  // of |v| on the far side
+    return v < 0.0f ? tail : 1.0f - tail;
+}
+
 // C values through the activation. One branch for all of them: with the branch inside, sixteen
 // copies of every function's code lay in the epilogue's loop, which then ran from instruction misses
 // (4099 x 4096 x 4096 without an activation 120 us, with a residual 331).
 template <uint32_t C>
-__device__ __forceinline__ void activate(float (&v)[C], uint32_t activation) {
+__device__ __forceinline__ void activate(float (&v)[C], uint32_t activation, bool short_out) {
     if (activation == LILY_ACT_NONE) {
     } else if (activation == LILY_ACT_RELU) {
 #pragma unroll
@@ -59,6 +75,11 @@ __device__ __forceinline__ void activate(float (&v)[C], uint32_t activation) {
 #pragma unroll
         for (uint32_t j = 0; j < C; ++j) {
             v[j] = __fdividef(v[j], 1.0f + expf(-v[j]));
+        }
+    } else if (activation == LILY_ACT_GELU && short_out) {
+#pragma unroll
+        for (uint32_t j = 0; j < C; ++j) {
+            v[j] *= normal_integral(v[j]);
         }
     } else if (activation == LILY_ACT_GELU) {
 #pragma unroll
@@ -116,11 +137,11 @@ __device__ __forceinline__ void residuals_of(const LinearArgs &a, const Output &
     }
 }
 
-// The sums v of output n and of up to C tokens from t on, finished and written. (A whole warp:
-// lane j has token j's scale.)
+// The sums v of an output and of up to C tokens from t on, finished; and written. (A whole warp: lane j
+// has token j's scale.)
 template <uint32_t C>
-__device__ __forceinline__ void finish(const LinearArgs &a, const Output &o, uint32_t t, uint32_t n, uint32_t live, float (&v)[C],
-                                       const float (&r)[C]) {
+__device__ __forceinline__ void finish_sums(const LinearArgs &a, const Output &o, uint32_t t, uint32_t live, float (&v)[C],
+                                            const float (&r)[C]) {
     if (a.a_scales != nullptr) {
         const uint32_t lane = threadIdx.x % 32u;
         const float mine = lane < min(live, C) ? __ldg(a.a_scales + t + lane) : 0.0f;
@@ -133,11 +154,17 @@ __device__ __forceinline__ void finish(const LinearArgs &a, const Output &o, uin
     for (uint32_t j = 0; j < C; ++j) {
         v[j] += o.bias;
     }
-    activate(v, a.activation);
+    activate(v, a.activation, !a.out_f32);
 #pragma unroll
     for (uint32_t j = 0; j < C; ++j) {
         v[j] += r[j];
     }
+}
+
+template <uint32_t C>
+__device__ __forceinline__ void finish(const LinearArgs &a, const Output &o, uint32_t t, uint32_t n, uint32_t live, float (&v)[C],
+                                       const float (&r)[C]) {
+    finish_sums(a, o, t, live, v, r);
     if (!o.live) {
     } else if (a.out_f32) {
         float *p = static_cast<float *>(a.out) + (uint64_t)t * a.out_ld + n;
@@ -519,29 +546,34 @@ __global__ void __launch_bounds__(192) linear_few_kernel(const __grid_constant__
 
 // ----------------------------------------------------------------- many tokens --
 //
-// Tiles of 256 outputs x 256 tokens, each by a pair of blocks (a cluster of two on neighbouring
-// SMs) whose tensor cores multiply together: either block holds 128 outputs' weights and 128 tokens in
+// Tiles of 256 outputs x up to 256 tokens, each by a pair of blocks (a cluster of two on neighbouring
+// SMs) whose tensor cores multiply together: either block holds 128 outputs' weights and half of the tokens in
 // shared memory, and the pair's multiply reads both. That halves the bytes that a multiply takes
 // out of each SM's shared memory, which one block alone is bound by. The pairs stay for all of the launch; an
 // accumulator is finished (scale, bias, activation, residual) while the next tile is multiplied
-// into the other one.
+// into the other one. bf16 outs and residuals go through shared memory where their rows allow it: the
+// residuals come while the tile is multiplied, and nothing in the epilogue waits for global memory. (Read
+// and written in place, 64 bytes a warp at a time, they took 55 us of the 153 of 4099 x 4096 x 4096.)
 //
 // A block's warps: 0 asks for the block's copies, 1 issues the pair's multiplies (in the first block
 // of the pair alone), 2 to 9 are the epilogue, two for each quarter of tensor memory's lanes.
 struct Many {
     static constexpr uint32_t THREADS = 320;
-    static constexpr uint32_t TILE = 256;          // of outputs and of tokens
-    static constexpr uint32_t STAGES = 6;
+    static constexpr uint32_t TILE = 256;          // of outputs, and the most of tokens
+    static constexpr uint32_t STAGES = 5;
     static constexpr uint32_t STAGE = 2u * A_STAGE;  // a block's half of the weights, and of the tokens
+    static constexpr uint32_t WARP_TILE = 128u * 64u;  // bf16 outs of a warp of the epilogue: 128 tokens, 32 outputs
     static constexpr uint32_t ACCS = 2;
     static constexpr uint32_t EPI_WARPS = 8;
     static constexpr uint32_t COLS = ACCS * TILE;
-    static constexpr uint32_t FULL_BARS = STAGES * STAGE;           // in the first block: both blocks' copies are there
+    static constexpr uint32_t OUT = STAGES * STAGE;
+    static constexpr uint32_t FULL_BARS = OUT + EPI_WARPS * WARP_TILE;  // in the first block: both blocks' copies are there
     static constexpr uint32_t EMPTY = FULL_BARS + 8u * STAGES;
     static constexpr uint32_t ACC_FULL = EMPTY + 8u * STAGES;
     static constexpr uint32_t ACC_EMPTY = ACC_FULL + 8u * ACCS;     // in the first block: both blocks have read it
     static constexpr uint32_t FINAL = ACC_EMPTY + 8u * ACCS;
-    static constexpr uint32_t TMEM_ADDR = FINAL + 8u;
+    static constexpr uint32_t RESIDUAL = FINAL + 8u;                // [EPI_WARPS] the warp's residuals are there
+    static constexpr uint32_t TMEM_ADDR = RESIDUAL + 8u * EPI_WARPS;
     static constexpr uint32_t ABORT = TMEM_ADDR + 4u;
     static constexpr uint32_t BYTES = ABORT + 4u + 1024u;
     static_assert(BYTES <= 227u * 1024u, "shared memory of one block");
@@ -553,6 +585,13 @@ __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap
         "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
         ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(cluster_bar), "r"(x), "r"(y)
         : "memory");
+}
+
+// A tile out of shared memory; parts beyond the tensor are left out.
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap *map, uint32_t src, int32_t x, int32_t y) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];"
+                 ::"l"(reinterpret_cast<uint64_t>(map)), "r"(src), "r"(x), "r"(y)
+                 : "memory");
 }
 
 template <bool E4M3>
@@ -605,6 +644,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(320, 1) linear_many_
             mbar_init(base + S::ACC_EMPTY + 8 * b, 2u * S::EPI_WARPS);
         }
         mbar_init(base + S::FINAL, 1);
+        for (uint32_t w = 0; w < S::EPI_WARPS; ++w) {
+            mbar_init(base + S::RESIDUAL + 8 * w, 1);
+        }
         *abort_word = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -629,7 +671,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(320, 1) linear_many_
             bool gave_up = false;
             for (uint32_t tile = pair; tile < tiles && !gave_up; tile += pairs) {
                 const int32_t output0 = (int32_t)(tile / a.token_tiles * S::TILE + rank * TILE_M);
-                const int32_t token0 = (int32_t)(tile % a.token_tiles * S::TILE + rank * TILE_M);
+                const int32_t token0 = (int32_t)(tile % a.token_tiles * a.tile_tokens + rank * (a.tile_tokens / 2u));
                 for (uint32_t k = 0; k < a.blocks; ++k, ++i) {
                     const uint32_t s = i % S::STAGES;
                     if (mbar_wait(base + S::EMPTY + 8 * s, (i / S::STAGES & 1u) ^ 1u, abort_word, a.wait_ns)) {
@@ -642,7 +684,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(320, 1) linear_many_
                         continue;  // (test hook: the stage never fills)
                     }
                     if (rank == 0u) {
-                        mbar_expect_tx(bar, 2u * S::STAGE);
+                        mbar_expect_tx(bar, 2u * A_STAGE + a.tile_tokens * BLOCK_BYTES);
                     }
                     tma_load_2d_pair(to, &a.w_map, at_rank(bar, 0), x, output0);
                     tma_load_2d_pair(to + A_STAGE, &a.a_map, at_rank(bar, 0), x, token0);
@@ -658,7 +700,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(320, 1) linear_many_
         __syncwarp();
     } else if (warp == 1u && rank == 0u) {
         const bool leader = elect_one();
-        const uint32_t idesc = product_desc<E4M3>(2u * TILE_M, S::TILE);
+        const uint32_t idesc = product_desc<E4M3>(2u * TILE_M, a.tile_tokens);
         uint32_t i = 0, turn = 0;
         bool gave_up = false;
         for (uint32_t tile = pair; tile < tiles && !gave_up; tile += pairs, ++turn) {
@@ -695,34 +737,89 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(320, 1) linear_many_
         __syncwarp();
     } else if (warp >= 2u) {
         const uint32_t quad = warp % 4u, half = (warp - 2u) / 4u;
-        uint32_t turn = 0;
+        uint32_t turn = 0, loaded = 0;  // tiles; residuals asked for
         for (uint32_t tile = pair; tile < tiles; tile += pairs, ++turn) {
             const uint32_t b = turn % S::ACCS;
             const uint32_t n = tile / a.token_tiles * S::TILE + rank * TILE_M + quad * 32u + lane;
-            const uint32_t token0 = tile % a.token_tiles * S::TILE + half * (S::TILE / 2u);
-            const uint32_t live = token0 < a.tokens ? min(S::TILE / 2u, a.tokens - token0) : 0u;
-            const uint32_t from = tmem + (quad * 32u << 16) + b * S::TILE + half * (S::TILE / 2u);
+            const uint32_t tokens = a.tile_tokens / 2u, token0 = tile % a.token_tiles * a.tile_tokens + half * tokens;
+            const uint32_t live = token0 < a.tokens ? min(tokens, a.tokens - token0) : 0u;
+            const uint32_t from = tmem + (quad * 32u << 16) + b * S::TILE + half * tokens;
             const Output o = output_of(a, n);
-            float r[16];
-            residuals_of(a, o, token0, n, live, r);
-            if (warp_wait(base + S::ACC_FULL + 8 * b, turn / S::ACCS & 1u, abort_word, a.wait_ns)) {
-                break;
-            }
-            tc_fence_after();
-            for (uint32_t c = 0; c < live; c += 16u) {
-                uint32_t q[16];
-                float v[16], next[16];
-                tmem_ld16(from + c, q);
-                residuals_of(a, o, token0 + c + 16u, n, live > c + 16u ? live - c - 16u : 0u, next);  // (asked for a round ahead)
-                tmem_ld_wait();
-#pragma unroll
-                for (uint32_t j = 0; j < 16u; ++j) {
-                    v[j] = __uint_as_float(q[j]);
+            if (a.copies) {
+                const uint32_t w = warp - 2u, mine = base + S::OUT + w * S::WARP_TILE + lane * 2u, bar = base + S::RESIDUAL + 8 * w;
+                const bool any = live > 0u && n - lane < a.outputs;
+                if (any && lane == 0u) {
+                    asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // (the last tile's outs have left)
+                    if (a.residual != nullptr) {
+                        mbar_expect_tx(bar, tokens * 64u);
+                        tma_load_2d(mine, &a.residual_map, bar, (int32_t)n, (int32_t)token0);
+                        ++loaded;
+                    }
                 }
-                finish(a, o, token0 + c, n, live - c, v, r);
+                __syncwarp();
+                if (warp_wait(base + S::ACC_FULL + 8 * b, turn / S::ACCS & 1u, abort_word, a.wait_ns)) {
+                    break;
+                }
+                tc_fence_after();
+                loaded = __shfl_sync(FULL, loaded, 0);
+                if (any && a.residual != nullptr && warp_wait(bar, (loaded - 1u) & 1u, abort_word, a.wait_ns)) {
+                    break;
+                }
+                for (uint32_t c = 0; any && c < live; c += 16u) {
+                    uint32_t q[16];
+                    float v[16], r[16];
+                    tmem_ld16(from + c, q);
 #pragma unroll
-                for (uint32_t j = 0; j < 16u; ++j) {
-                    r[j] = next[j];
+                    for (uint32_t j = 0; j < 16u; ++j) {
+                        r[j] = 0.0f;
+                        if (a.residual != nullptr) {
+                            uint16_t x;
+                            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(x) : "r"(mine + (c + j) * 64u));
+                            r[j] = __uint_as_float((uint32_t)x << 16);
+                        }
+                    }
+                    tmem_ld_wait();
+#pragma unroll
+                    for (uint32_t j = 0; j < 16u; ++j) {
+                        v[j] = __uint_as_float(q[j]);
+                    }
+                    finish_sums(a, o, token0 + c, live - c, v, r);
+#pragma unroll
+                    for (uint32_t j = 0; j < 16u; ++j) {
+                        asm volatile("st.shared.u16 [%0], %1;" ::"r"(mine + (c + j) * 64u), "h"(__bfloat16_as_ushort(__float2bfloat16_rn(v[j])))
+                                     : "memory");
+                    }
+                }
+                if (any) {
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0u) {
+                        tma_store_2d(&a.out_map, mine, (int32_t)n, (int32_t)token0);
+                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                    }
+                }
+            } else {
+                float r[16];
+                residuals_of(a, o, token0, n, live, r);
+                if (warp_wait(base + S::ACC_FULL + 8 * b, turn / S::ACCS & 1u, abort_word, a.wait_ns)) {
+                    break;
+                }
+                tc_fence_after();
+                for (uint32_t c = 0; c < live; c += 16u) {
+                    uint32_t q[16];
+                    float v[16], next[16];
+                    tmem_ld16(from + c, q);
+                    residuals_of(a, o, token0 + c + 16u, n, live > c + 16u ? live - c - 16u : 0u, next);  // (asked for a round ahead)
+                    tmem_ld_wait();
+#pragma unroll
+                    for (uint32_t j = 0; j < 16u; ++j) {
+                        v[j] = __uint_as_float(q[j]);
+                    }
+                    finish(a, o, token0 + c, n, live - c, v, r);
+#pragma unroll
+                    for (uint32_t j = 0; j < 16u; ++j) {
+                        r[j] = next[j];
+                    }
                 }
             }
             tc_fence_before();
@@ -733,6 +830,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(320, 1) linear_many_
                              : "memory");
             }
         }
+        // (Nothing is on its way to or from this block's shared memory when it ends: outs here; residuals that
+        // nobody waited for, if it has given up.)
+        if (lane == 0u) {
+            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            if (*abort_word && loaded > 0u) {
+                mbar_drain(base + S::RESIDUAL + 8 * (warp - 2u), (loaded - 1u) & 1u, a.wait_ns);
+            }
+        }
+        __syncwarp();
     }
 
     tc_fence_before();
@@ -826,6 +932,17 @@ bool encode_rows(CUtensorMap *map, const void *p, uint64_t ld, uint32_t rows, ui
                                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// bf16 outs or residuals, in boxes of `tokens` x 32 outputs.
+bool encode_outs(CUtensorMap *map, const void *p, uint64_t ld, const lily_linear_args_t &g, uint32_t tokens) {
+    const cuuint64_t dims[2] = {g.outputs, g.tokens};
+    const cuuint64_t strides[1] = {ld * 2u};
+    const cuuint32_t box[2] = {32u, tokens};
+    const cuuint32_t estr[2] = {1, 1};
+    return tensor_map_encoder()(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void *>(p), dims, strides, box, estr,
+                                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 }  // namespace
 
 extern "C" int32_t lily_linear(lily_sampler_t *h, void *stream_, const lily_linear_args_t *args) {
@@ -888,15 +1005,41 @@ extern "C" int32_t lily_linear(lily_sampler_t *h, void *stream_, const lily_line
     h->lost_stage = 0xFFFFFFFFu;  // one launch only
 
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-    const uint64_t big_tiles = (uint64_t)((g.tokens + Many::TILE - 1u) / Many::TILE) * ((g.outputs + Many::TILE - 1u) / Many::TILE);
-    if (g.tokens > 256u && big_tiles <= 0x7FFFFFFFull) {
-        if (!encode_rows(&a.w_map, g.weight, g.weight_ld, g.outputs, g.columns, g.dtype, TILE_M) ||
-            !encode_rows(&a.a_map, g.a, g.a_ld, g.tokens, g.columns, g.dtype, TILE_M)) {
-            return fail(h, LILY_ERR_CUDA, "cuTensorMapEncodeTiled refused a or weight");
+    // Pairs of blocks above 128 tokens, unless the tiles would leave half of the SMs idle and the columns are long
+    // enough to be shared: 64 steps. Pairs do not share columns (pairs, and single blocks that share, in us:
+    // 256 x 2048 x 11000 19 and 24, 640 x 4096 x 4096 24 and 37, 1024 x 1024 x 1024 8.6 and 10.7; the other
+    // way 256 x 4096 x 4096 22 and 17, 300 x 8192 x 2048 38 and 23, 1024 x 4096 x 1024 21 and 16).
+    const uint64_t sms = (uint32_t)h->sm_count;
+    const uint64_t singles = (g.tokens + 127ull) / 128u * ((g.outputs + TILE_M - 1ull) / TILE_M);
+    if (g.tokens > 128u && (singles * 2u > sms || a.blocks < 64u)) {
+        // The tile's tokens: the shortest way for the busiest pair. A smaller tile costs little less than one of
+        // 256 tokens (4099 x 4096 x 4096: five of 192 in turn 107 us, four of 256 96 to 98; 8192 x 8192 x 4096:
+        // 544 and 409): what is read for a tile, the weights above all, stays.
+        const uint64_t pairs = sms / 2u, output_tiles = (g.outputs + Many::TILE - 1ull) / Many::TILE;
+        uint64_t best = ~0ull;
+        for (uint32_t t = Many::TILE; t >= 64u; t -= 32u) {
+            const uint64_t tiles = (g.tokens + t - 1u) / t * output_tiles, cost = (tiles + pairs - 1u) / pairs * (t + 320u);
+            if (cost < best) {
+                best = cost;
+                a.tile_tokens = t;
+            }
         }
-        a.token_tiles = (g.tokens + Many::TILE - 1u) / Many::TILE;
-        const uint32_t pairs = (uint32_t)std::min<uint64_t>(big_tiles, (uint32_t)h->sm_count / 2u);
-        CU(h, e4m3 ? launch_many<true>(a, pairs, stream) : launch_many<false>(a, pairs, stream));
+        a.token_tiles = (g.tokens + a.tile_tokens - 1u) / a.tile_tokens;
+        const uint64_t tiles = a.token_tiles * output_tiles;
+        if (tiles > 0x7FFFFFFFull) {
+            return fail(h, LILY_ERR_CAPACITY, "more tiles than a launch takes");
+        }
+        const auto rows16 = [&](const void *p, uint64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16u == 0u && ld * 2u % 16u == 0u; };
+        // (A copy out of shared memory writes whole 16 bytes: rows of 1003 outputs had zeroes behind them.)
+        a.copies = !a.out_f32 && g.outputs % 8u == 0u && rows16(g.out, g.out_ld) && (g.residual == nullptr || rows16(g.residual, g.residual_ld));
+        if (!encode_rows(&a.w_map, g.weight, g.weight_ld, g.outputs, g.columns, g.dtype, TILE_M) ||
+            !encode_rows(&a.a_map, g.a, g.a_ld, g.tokens, g.columns, g.dtype, a.tile_tokens / 2u) ||
+            (a.copies && (!encode_outs(&a.out_map, g.out, g.out_ld, g, a.tile_tokens / 2u) ||
+                          (g.residual != nullptr && !encode_outs(&a.residual_map, g.residual, g.residual_ld, g, a.tile_tokens / 2u))))) {
+            return fail(h, LILY_ERR_CUDA, "cuTensorMapEncodeTiled refused a, weight, out or residual");
+        }
+        const uint32_t used = (uint32_t)std::min(tiles, pairs);
+        CU(h, e4m3 ? launch_many<true>(a, used, stream) : launch_many<false>(a, used, stream));
         return LILY_OK;
     }
     const uint32_t n = g.tokens <= 16u ? 16u : g.tokens <= 32u ? 32u : g.tokens <= 64u ? 64u : 128u;
@@ -912,7 +1055,6 @@ extern "C" int32_t lily_linear(lily_sampler_t *h, void *stream_, const lily_line
     // Shares of the columns: as many blocks as there are SMs, of four steps at least; up to 32 tokens two on
     // an SM, of eight (24 x 4096 x 4096: e4m3, four shares of eight steps 7.7 us, eight of four 8.2; bf16, of
     // sixteen 10.6, of eight 9.4; 64 tokens on one block an SM 12.7 us, on two 14.1).
-    const uint64_t sms = (uint32_t)h->sm_count;
     uint32_t shares = 8u;
     while (shares > 1u && (tiles * shares > sms * (n <= 32u ? 2u : 1u) || a.blocks < (tiles * shares > sms ? 8u : 4u) * shares)) {
         shares /= 2u;

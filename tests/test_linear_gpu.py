@@ -109,6 +109,73 @@ def test_epilogue(cuda, lily, act, tokens, columns, outputs):
 
 
 @pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("tokens,columns,outputs", [(129, 128, 9480), (200, 72, 9600), (301, 512, 520), (385, 4096, 4096),
+                                                    (600, 256, 1032), (1030, 1024, 256), (2500, 64, 1224), (300, 4096, 512),
+                                                    (333, 128, 1003), (450, 64, 9481)])
+def test_many_tokens_with_rows_on_boundaries(cuda, lily, kind, tokens, columns, outputs):
+    """bf16 outs and residuals whose rows start on 16-byte boundaries: contiguous, as a part of wider rows, in
+    place; tiles that end inside the tokens and the outputs leave what lies behind them."""
+    torch = cuda
+    g = torch.Generator(device="cuda").manual_seed(tokens + outputs)
+    scratch = _handle(lily)
+    a, w, kw = _inputs(torch, g, tokens, columns, outputs, kind)
+    pitch = (outputs + 7) // 8 * 8
+    for act, bias_type, wide, with_residual in (("none", None, 0, False), ("silu", torch.float32, 8, True),
+                                                ("gelu", torch.bfloat16, 40, True), ("relu", None, 0, True)):
+        bias = None if bias_type is None else torch.randn(outputs, generator=g, device="cuda").to(bias_type)
+        residual = None
+        if with_residual:
+            residual = torch.randn((tokens, pitch + 2 * wide), generator=g, device="cuda").bfloat16()[:, wide:wide + outputs]
+        out = torch.full((tokens + 2, pitch + 2 * wide), 3.0, dtype=torch.bfloat16, device="cuda")
+        mine = out[1:-1, wide:wide + outputs]
+        scratch.linear(a, w, mine, bias=bias, activation=act, residual=residual, **kw)
+        _check(torch, mine, a, w, kw, bias, act, residual)
+        assert (out[0] == 3).all() and (out[-1] == 3).all()
+        assert (out[:, :wide] == 3).all() and (out[:, wide + outputs:] == 3).all()
+        if residual is not None:
+            place = torch.full_like(out, 3.0)
+            mine2 = place[1:-1, wide:wide + outputs]
+            mine2.copy_(residual)
+            scratch.linear(a, w, mine2, bias=bias, activation=act, residual=mine2, **kw)
+            assert torch.equal(place, out)
+    assert scratch.status() == lily.OK
+
+
+def test_rows_on_boundaries_and_off_them_give_the_same(cuda, lily):
+    torch = cuda
+    g = torch.Generator(device="cuda").manual_seed(21)
+    scratch = _handle(lily)
+    a, w, kw = _inputs(torch, g, 700, 512, 1024, "bf16")
+    residual = torch.randn((700, 1024), generator=g, device="cuda").bfloat16()
+    out = torch.empty((700, 1024), dtype=torch.bfloat16, device="cuda")
+    odd = torch.empty((700, 1025), dtype=torch.bfloat16, device="cuda")[:, 1:]
+    odd_residual = torch.empty((700, 1027), dtype=torch.bfloat16, device="cuda")[:, 2:1026].copy_(residual)
+    for act in ("none", "silu", "gelu", "gelu_tanh"):
+        scratch.linear(a, w, out, activation=act, residual=residual)
+        scratch.linear(a, w, odd, activation=act, residual=odd_residual)
+        assert torch.equal(out, odd)
+
+
+def test_lost_copy_with_a_residual(cuda, lily):
+    """The residual's copies are under way when the wait runs out; the next call is right."""
+    torch = cuda
+    g = torch.Generator(device="cuda").manual_seed(22)
+    scratch = _handle(lily)
+    a, w, kw = _inputs(torch, g, 900, 1024, 2048, "bf16")
+    residual = torch.randn((900, 2048), generator=g, device="cuda").bfloat16()
+    out = torch.empty_like(residual)
+    for stage in (0, 3, 15):
+        scratch.set_wait_limit(20_000_000)
+        scratch.inject_lost_copy(stage)
+        scratch.linear(a, w, out, residual=residual)
+        assert scratch.status() == lily.ERR_TIMEOUT
+        scratch.set_wait_limit(0)
+        scratch.linear(a, w, out, residual=residual)
+        assert scratch.status() == lily.OK
+        _check(torch, out, a, w, kw, residual=residual)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
 def test_exact_where_the_sums_are(cuda, lily, kind):
     """Small integers: every partial sum is exact in binary32, in any order and any shares."""
     torch = cuda
