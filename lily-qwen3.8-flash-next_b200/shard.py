@@ -83,13 +83,18 @@ def gather_records(local_records, group=None):
 
 def sharded_lmhead_draw(scratch, weights, scales, hidden, params, out_ids, first_id: int, *,
                         uniforms=None, steps=None, records=None, want_sums: bool = False,
-                        out_lse=None, group=None, stream=None, exchange=None, **kept):
+                        out_lse=None, group=None, stream=None, exchange=None, adjust=None, logits=None, **kept):
     """One vocab-sharded step on this rank: the 8-bit head over this rank's
     rows and its candidate records (lily_lmhead_shard_candidates), the
     all-gather of the records, the merged draw (lily_merge_draw). Every rank
     ends with the same token ids in `out_ids`. `scratch` was created with
     lmhead=True for this rank's shard size. With `exchange` (a PeerExchange) the
-    all-gather is the ranks' own stores into each other's memory instead."""
+    all-gather is the ranks' own stores into each other's memory instead.
+
+    With `adjust`, a dict of keywords of SamplerScratch.adjust_logits (mask, history_ids,
+    bias_ids, ... by the whole vocabulary's ids, the same on every rank), the shard's logits
+    are written to `logits` (f32 [rows, shard], allocated if None), adjusted there with the penalties of
+    `params`, and drawn from without them."""
     import contextlib
 
     import torch
@@ -97,21 +102,36 @@ def sharded_lmhead_draw(scratch, weights, scales, hidden, params, out_ids, first
     rows = hidden.shape[0]
     if records is None:
         records = torch.empty((rows, RECORD_BYTES), dtype=torch.uint8, device=hidden.device)
+    on_stream = torch.cuda.stream(stream) if (stream is not None and hidden.is_cuda) else contextlib.nullcontext()
+    if adjust is not None:
+        import lily_b200 as lily
+
+        with_penalties, params = params, [lily.draft_params(p) for p in params]
+        if logits is None:
+            with on_stream:  # (the stream's own memory: free for others when its work is done)
+                logits = torch.empty((rows, weights.shape[0]), device=hidden.device)
+
+    def candidates():
+        if adjust is None:
+            scratch.lmhead_shard_candidates(weights, scales, hidden, params, records, first_id=first_id,
+                                            want_sums=want_sums, stream=stream)
+            return
+        scratch.lmhead_logits(weights, scales, hidden, logits, stream=stream)
+        scratch.adjust_logits(logits, with_penalties, first_id=first_id, stream=stream, **adjust)
+        scratch.shard_candidates(logits, params, records, first_id=first_id, want_sums=want_sums, stream=stream)
+
     if exchange is not None:
         # No collective library on the data path: the records go straight into the
         # other ranks' memory, and the merge waits for their flags.
-        scratch.lmhead_shard_candidates(weights, scales, hidden, params, records, first_id=first_id,
-                                        want_sums=want_sums, stream=stream)
+        candidates()
         exchange.publish_and_merge(scratch, records, params, out_ids, uniforms=uniforms, steps=steps,
                                    out_lse=out_lse, stream=stream, **kept)
         return None
     # The collective is ordered against torch's CURRENT stream only: a stream
     # that is given is made current for the whole step, so that the records are
     # written before the all-gather reads them and gathered before the merge.
-    current = torch.cuda.stream(stream) if (stream is not None and hidden.is_cuda) else contextlib.nullcontext()
-    with current:
-        scratch.lmhead_shard_candidates(weights, scales, hidden, params, records, first_id=first_id,
-                                        want_sums=want_sums, stream=stream)
+    with on_stream:
+        candidates()
         gathered = gather_records(records, group=group)
         scratch.merge_draw(gathered, params, out_ids, uniforms=uniforms, steps=steps, out_lse=out_lse,
                            stream=stream, **kept)
