@@ -84,9 +84,13 @@ enum lily_activation {
  * Any numbers of tokens, outputs and columns. The rows of a and weight start on 16-byte
  * boundaries (their pitches multiples of 16 bytes); out, bias and residual need no alignment
  * beyond their elements'. `residual` may be `out` itself (the same address and pitch); else out
- * overlaps no other buffer. A token's results do not depend on the tokens beside it as long as
- * their number stays within the same of the ranges 1..16, ..32, ..64, ..128 and above (a larger
- * call may add up its columns in other shares).
+ * overlaps no other buffer. A call gives the same bits every time, and a token's do not depend
+ * on the tokens beside it; up to 64 tokens they do not depend on their number either as long as
+ * that stays within 1..16, ..32 or ..64. (The columns are added up in shares whose number is
+ * chosen by the sizes.)
+ *
+ * The first call of a kind loads its kernel (up to 16, 32, 64 tokens and more; BF16 or E4M3):
+ * make it before a capture.
  */
 typedef struct lily_linear_args {
     uint32_t struct_size;    /* sizeof(lily_linear_args_t) */

@@ -364,7 +364,9 @@ int32_t lily_argmax_batch(lily_sampler_t *h, void *stream, const void *logits,
  * params are invalid, is left as it was (in `out` too): status LILY_ROW_LIST / LILY_ROW_PARAMS,
  * and the handle's sticky status. A row whose mask index is not below `masks` counts as LIST.
  *
- * Nothing of the handle is written but the status word: calls may overlap on the GPU.
+ * Nothing of the handle is written but the status word: calls may overlap on the GPU. Masks
+ * take ids up to 2^31 - 1 (LILY_ERR_CAPACITY beyond). The first call of a kind (masks and bans
+ * alone, or any other list) loads its kernel: make it before a capture.
  */
 typedef struct lily_adjust_args {
     uint32_t struct_size;        /* sizeof(lily_adjust_args_t) */
@@ -532,7 +534,8 @@ int32_t lily_lmhead_logits(lily_sampler_t *h, void *stream, const lily_lmhead_t 
  *
  * Limits: params are HOST arrays; sampled rows need 1 <= top_k <= 64; no
  * penalties, bias, ban or forced ids (their ids would be global, the shard's
- * logits are local): refused with LILY_ERR_ARG.
+ * logits are local): refused with LILY_ERR_ARG. A shard's logits get them, and
+ * masks, from lily_adjust_logits before lily_shard_candidates reads them.
  */
 #define LILY_SHARD_CANDIDATES 64u
 #define LILY_SHARD_RECORD_BYTES 520u

@@ -41,6 +41,8 @@ struct LinearArgs {
     uint32_t token_tiles;
     uint32_t tile_tokens;   // many tokens: of a tile, a multiple of 32
     uint32_t copies;        // many tokens: out and residual go through shared memory
+    uint32_t shares;        // many tokens: pairs of a cluster that share a tile's columns
+    uint32_t stages;        // many tokens: of the pipeline
     uint32_t out_f32, bias_f32, activation;
     uint32_t *status_word;
     uint64_t wait_ns;
@@ -137,17 +139,31 @@ __device__ __forceinline__ void residuals_of(const LinearArgs &a, const Output &
     }
 }
 
-// The sums v of an output and of up to C tokens from t on, finished; and written. (A whole warp: lane j
-// has token j's scale.)
+// The scales of up to 128 tokens from t on, token 32 i + j's with lane j: asked for before the sums are there.
+struct TokenScales {
+    float v[4];
+
+    __device__ __forceinline__ TokenScales(const LinearArgs &a, uint32_t t, uint32_t live) {
+        const uint32_t lane = threadIdx.x % 32u;
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; ++i) {
+            v[i] = a.a_scales != nullptr && 32u * i + lane < live ? __ldg(a.a_scales + t + 32u * i + lane) : 0.0f;
+        }
+    }
+
+    __device__ __forceinline__ float of(uint32_t c) const { return c < 64u ? (c < 32u ? v[0] : v[1]) : c < 96u ? v[2] : v[3]; }
+};
+
+// The sums v of an output and of C tokens from the c-th of `s` on (all of them among the same 32), finished; and
+// written, up to `live` of them. (A whole warp.)
 template <uint32_t C>
-__device__ __forceinline__ void finish_sums(const LinearArgs &a, const Output &o, uint32_t t, uint32_t live, float (&v)[C],
+__device__ __forceinline__ void finish_sums(const LinearArgs &a, const Output &o, const TokenScales &s, uint32_t c, float (&v)[C],
                                             const float (&r)[C]) {
     if (a.a_scales != nullptr) {
-        const uint32_t lane = threadIdx.x % 32u;
-        const float mine = lane < min(live, C) ? __ldg(a.a_scales + t + lane) : 0.0f;
+        const float mine = s.of(c);
 #pragma unroll
         for (uint32_t j = 0; j < C; ++j) {
-            v[j] *= __shfl_sync(FULL, mine, j) * o.scale;
+            v[j] *= __shfl_sync(FULL, mine, c % 32u + j) * o.scale;
         }
     }
 #pragma unroll
@@ -162,9 +178,9 @@ __device__ __forceinline__ void finish_sums(const LinearArgs &a, const Output &o
 }
 
 template <uint32_t C>
-__device__ __forceinline__ void finish(const LinearArgs &a, const Output &o, uint32_t t, uint32_t n, uint32_t live, float (&v)[C],
-                                       const float (&r)[C]) {
-    finish_sums(a, o, t, live, v, r);
+__device__ __forceinline__ void finish(const LinearArgs &a, const Output &o, const TokenScales &s, uint32_t c, uint32_t t, uint32_t n,
+                                       uint32_t live, float (&v)[C], const float (&r)[C]) {
+    finish_sums(a, o, s, c, v, r);
     if (!o.live) {
     } else if (a.out_f32) {
         float *p = static_cast<float *>(a.out) + (uint64_t)t * a.out_ld + n;
@@ -234,14 +250,14 @@ struct Few {
     static constexpr uint32_t B_STAGE = N * BLOCK_BYTES;
     static constexpr uint32_t STAGE = A_STAGE + B_STAGE;
     static constexpr uint32_t PART_BYTES = N * TILE_M * 4u;
-    // Two blocks on an SM up to 64 tokens, else one.
-    static constexpr uint32_t STAGES = N == 16u ? 5u : N == 32u ? 4u : N == 64u ? 4u : 6u;
+    // Two blocks on an SM.
+    static constexpr uint32_t STAGES = N == 16u ? 5u : 4u;
     // The sums that blocks send one another have a place of their own (a block may send as soon as the
     // other runs), or, where that takes a stage, the stages' (it has to be done with its columns).
     static constexpr bool OVER_STAGES = N >= 64u;
     // Sums of successive steps go into accumulators in turn: shorter chains of additions. Two sets of them: a
     // tile is finished while the block's next one is multiplied.
-    static constexpr uint32_t ACCS = N <= 64u ? 2u : 1u, SETS = 2;
+    static constexpr uint32_t ACCS = 2, SETS = 2;
     static constexpr uint32_t COLS = SETS * ACCS * N;
     static constexpr uint32_t PART = OVER_STAGES ? 0u : STAGES * STAGE;
     static constexpr uint32_t BARS = STAGES * STAGE + (OVER_STAGES ? 0u : PART_BYTES);
@@ -269,9 +285,8 @@ __global__ void __launch_bounds__(192) linear_few_kernel(const __grid_constant__
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(shares));
     const uint32_t tile0 = blockIdx.x / shares, stride = gridDim.x / shares;
-    const uint32_t tiles = (a.outputs + TILE_M - 1u) / TILE_M * a.token_tiles;
-    const auto token_of = [&](uint32_t tile) { return tile % a.token_tiles * N; };
-    const auto output_tile = [&](uint32_t tile) { return tile / a.token_tiles * TILE_M; };
+    const uint32_t tiles = (a.outputs + TILE_M - 1u) / TILE_M;
+    const auto output_tile = [&](uint32_t tile) { return tile * TILE_M; };
     const uint32_t block0 = (uint32_t)((uint64_t)a.blocks * rank / shares);
     const uint32_t steps = (uint32_t)((uint64_t)a.blocks * (rank + 1u) / shares) - block0;
 
@@ -310,7 +325,7 @@ __global__ void __launch_bounds__(192) linear_few_kernel(const __grid_constant__
         if (lane == 0u) {
             uint32_t asked = 0, parity = 0, i = 0;
             for (uint32_t tile = tile0; tile < tiles; tile += stride) {
-                const int32_t token0 = (int32_t)token_of(tile), output0 = (int32_t)output_tile(tile);
+                const int32_t output0 = (int32_t)output_tile(tile);
                 for (uint32_t k = 0; k < steps; ++k, ++i) {
                     const uint32_t s = i % S::STAGES, use = i / S::STAGES;
                     if (mbar_wait(base + S::EMPTY + 8 * s, (use & 1u) ^ 1u, abort_word, a.wait_ns)) {
@@ -326,7 +341,7 @@ __global__ void __launch_bounds__(192) linear_few_kernel(const __grid_constant__
                     parity = (parity & ~(1u << s)) | (use & 1u) << s;
                     mbar_expect_tx(bar, S::STAGE);
                     tma_load_2d(to, &a.w_map, bar, x, output0);
-                    tma_load_2d(to + A_STAGE, &a.a_map, bar, x, token0);
+                    tma_load_2d(to + A_STAGE, &a.a_map, bar, x, 0);
                 }
             }
             if (*abort_word) {  // the copies asked for land in this block's shared memory: it stays until they have
@@ -406,17 +421,18 @@ __global__ void __launch_bounds__(192) linear_few_kernel(const __grid_constant__
     if (shares == 1u) {
         uint32_t turn = 0;
         for (uint32_t tile = tile0; warp >= 2u && tile < tiles; tile += stride, ++turn) {
-            const uint32_t b = turn % S::SETS, token0 = token_of(tile), n = output_tile(tile) + row, live = min(N, a.tokens - token0);
+            const uint32_t b = turn % S::SETS, n = output_tile(tile) + row, live = a.tokens;
             const Output o = output_of(a, n);
+            const TokenScales scales(a, 0u, live);
             float r[16];
-            residuals_of(a, o, token0, n, live, r);  // (asked for a round ahead, here and below)
+            residuals_of(a, o, 0u, n, live, r);  // (asked for a round ahead, here and below)
             if (warp_wait(base + S::ACC_FULL + 8 * b, turn / S::SETS & 1u, abort_word, a.wait_ns)) {
                 break;
             }
             tc_fence_after();
             for (uint32_t c = 0; c < live; c += 16u) {
                 float v[16], next[16];
-                residuals_of(a, o, token0 + c + 16u, n, live > c + 16u ? live - c - 16u : 0u, next);
+                residuals_of(a, o, c + 16u, n, live > c + 16u ? live - c - 16u : 0u, next);
                 sums_of(b, c, v);
                 if (c + 16u >= live) {  // (the sums are in registers)
                     tc_fence_before();
@@ -425,7 +441,7 @@ __global__ void __launch_bounds__(192) linear_few_kernel(const __grid_constant__
                         mbar_arrive(base + S::ACC_EMPTY + 8 * b);
                     }
                 }
-                finish(a, o, token0 + c, n, live - c, v, r);
+                finish(a, o, scales, c, c, n, live - c, v, r);
 #pragma unroll
                 for (uint32_t j = 0; j < 16u; ++j) {
                     r[j] = next[j];
@@ -435,8 +451,8 @@ __global__ void __launch_bounds__(192) linear_few_kernel(const __grid_constant__
     } else {
         // Token c is finished by block c / per; its sums lie there at [share][output][c % per], four tokens
         // (or both) side by side, which an output's thread sends and takes together. (One by one the
-        // sums of 128 tokens took 3.6 us to send and 13 to add up.)
-        const uint32_t token0 = token_of(tile0), n = output_tile(tile0) + row, live = min(N, a.tokens - token0);
+        // sums of 128 tokens took 3.6 us to send and 13 to add up; the pairs have those now.)
+        const uint32_t n = output_tile(tile0) + row, live = a.tokens;
         const uint32_t per = N / shares, log_per = 31u - __clz(per);  // (powers of two)
         const uint32_t first = rank * per, mine = first < live ? min(per, live - first) : 0u;
         const uint32_t quads = per / 4u;
@@ -445,10 +461,11 @@ __global__ void __launch_bounds__(192) linear_few_kernel(const __grid_constant__
         };
         // What does not depend on the sums is asked for before they are there.
         Output o = {1.0f, 0.0f, false};
+        const TokenScales scales(a, first, warp >= 2u ? mine : 0u);
         float r[16];
         if (warp >= 2u) {
             o = output_of(a, n);
-            residuals_of(a, o, token0 + first, n, mine, r);
+            residuals_of(a, o, first, n, mine, r);
         }
         if (warp >= 2u) {
             warp_wait(base + S::ACC_FULL, 0u, abort_word, a.wait_ns);
@@ -497,7 +514,7 @@ __global__ void __launch_bounds__(192) linear_few_kernel(const __grid_constant__
                     v[0] += p.x, v[1] += p.y;
                 }
                 if (mine > 0u) {
-                    finish(a, o, token0 + first, n, mine, v, r2);
+                    finish(a, o, scales, 0u, first, n, mine, v, r2);
                 }
             } else {
                 const auto finish_all = [&](auto at_once) {
@@ -510,7 +527,7 @@ __global__ void __launch_bounds__(192) linear_few_kernel(const __grid_constant__
                                 rc[j] = r[j];
                             }
                         } else {
-                            residuals_of(a, o, token0 + first + c, n, mine - c, rc);
+                            residuals_of(a, o, first + c, n, mine - c, rc);
                         }
                         for (uint32_t k = 0; k < shares; ++k) {
 #pragma unroll
@@ -519,7 +536,7 @@ __global__ void __launch_bounds__(192) linear_few_kernel(const __grid_constant__
                                 v[j] += p.x, v[j + 1u] += p.y, v[j + 2u] += p.z, v[j + 3u] += p.w;
                             }
                         }
-                        finish(a, o, token0 + first + c, n, mine - c, v, rc);
+                        finish(a, o, scales, c, first + c, n, mine - c, v, rc);
                     }
                 };
                 if (per == 4u) {  // (no code for tokens that are not there: most of it runs once, and waits for itself)
@@ -546,7 +563,7 @@ __global__ void __launch_bounds__(192) linear_few_kernel(const __grid_constant__
 
 // ----------------------------------------------------------------- many tokens --
 //
-// Tiles of 256 outputs x up to 256 tokens, each by a pair of blocks (a cluster of two on neighbouring
+// From 65 tokens on. Tiles of 256 outputs x up to 256 tokens, each by a pair of blocks (a cluster of two on neighbouring
 // SMs) whose tensor cores multiply together: either block holds 128 outputs' weights and half of the tokens in
 // shared memory, and the pair's multiply reads both. That halves the bytes that a multiply takes
 // out of each SM's shared memory, which one block alone is bound by. The pairs stay for all of the launch; an
@@ -555,21 +572,29 @@ __global__ void __launch_bounds__(192) linear_few_kernel(const __grid_constant__
 // residuals come while the tile is multiplied, and nothing in the epilogue waits for global memory. (Read
 // and written in place, 64 bytes a warp at a time, they took 55 us of the 153 of 4099 x 4096 x 4096.)
 //
+// Where the tiles are few, two or four pairs of a cluster share the columns of one (256 x 8192 x 1024: 35 us
+// alone, 15 by four pairs). The stages are as many as fit beside the rest: few tokens make small ones.
+//
+// What bounds it: at 8192 x 4096 x 8192 (bf16 375 to 400 us, 1.4 PFLOP/s; e4m3 216 us, 2.5) and 4099 x 4096 x 4096
+// (96 to 104 us) the tiles that all SMs together take out of L2, 11 TB/s, and with the tensor cores
+// busy for three quarters of the time, the board's power; below about 1000 tokens the launch, the pipeline's
+// first copies and the last tile's end, 5 us together.
+//
 // A block's warps: 0 asks for the block's copies, 1 issues the pair's multiplies (in the first block
 // of the pair alone), 2 to 9 are the epilogue, two for each quarter of tensor memory's lanes.
 struct Many {
     static constexpr uint32_t THREADS = 320;
     static constexpr uint32_t TILE = 256;          // of outputs, and the most of tokens
-    static constexpr uint32_t STAGES = 5;
-    static constexpr uint32_t STAGE = 2u * A_STAGE;  // a block's half of the weights, and of the tokens
+    static constexpr uint32_t MOST_STAGES = 11;
+    static constexpr uint32_t RING = 5u * 2u * A_STAGE;  // bytes of stages: a block's half of the weights, and of the tokens
     static constexpr uint32_t WARP_TILE = 128u * 64u;  // bf16 outs of a warp of the epilogue: 128 tokens, 32 outputs
     static constexpr uint32_t ACCS = 2;
     static constexpr uint32_t EPI_WARPS = 8;
     static constexpr uint32_t COLS = ACCS * TILE;
-    static constexpr uint32_t OUT = STAGES * STAGE;
+    static constexpr uint32_t OUT = RING;          // (without outs and residuals in shared memory: stages, too)
     static constexpr uint32_t FULL_BARS = OUT + EPI_WARPS * WARP_TILE;  // in the first block: both blocks' copies are there
-    static constexpr uint32_t EMPTY = FULL_BARS + 8u * STAGES;
-    static constexpr uint32_t ACC_FULL = EMPTY + 8u * STAGES;
+    static constexpr uint32_t EMPTY = FULL_BARS + 8u * MOST_STAGES;
+    static constexpr uint32_t ACC_FULL = EMPTY + 8u * MOST_STAGES;
     static constexpr uint32_t ACC_EMPTY = ACC_FULL + 8u * ACCS;     // in the first block: both blocks have read it
     static constexpr uint32_t FINAL = ACC_EMPTY + 8u * ACCS;
     static constexpr uint32_t RESIDUAL = FINAL + 8u;                // [EPI_WARPS] the warp's residuals are there
@@ -577,6 +602,12 @@ struct Many {
     static constexpr uint32_t ABORT = TMEM_ADDR + 4u;
     static constexpr uint32_t BYTES = ABORT + 4u + 1024u;
     static_assert(BYTES <= 227u * 1024u, "shared memory of one block");
+
+    static constexpr uint32_t stage_bytes(uint32_t tokens) { return A_STAGE + tokens / 2u * BLOCK_BYTES; }
+    static constexpr uint32_t stages_of(uint32_t tokens, bool copies) {
+        const uint32_t n = (copies ? RING : FULL_BARS) / stage_bytes(tokens);
+        return n < MOST_STAGES ? n : MOST_STAGES;
+    }
 };
 
 // A copy into this block's shared memory whose bytes complete a barrier of either block of the pair.
@@ -613,29 +644,32 @@ __device__ __forceinline__ void mma_ss_pair(uint32_t d_tmem, uint64_t adesc, uin
     }
 }
 
-// Arrives at this barrier of both blocks once the multiplies issued so far have run.
-__device__ __forceinline__ void mma_commit_pair(uint32_t bar) {
+// Arrives at this barrier of both blocks of the pair, whose first in the cluster is `first`, once the multiplies issued so far have run.
+__device__ __forceinline__ void mma_commit_pair(uint32_t bar, uint32_t first) {
     asm volatile(
         "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
-        "h"((uint16_t)3)
+        "h"((uint16_t)(3u << first))
         : "memory");
 }
 
 template <bool E4M3>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(320, 1) linear_many_kernel(const __grid_constant__ LinearArgs a) {
+__global__ void __launch_bounds__(320, 1) linear_many_kernel(const __grid_constant__ LinearArgs a) {
     using S = Many;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t *smem = smem_raw + (base - smem_u32(smem_raw));
     volatile uint32_t *abort_word = reinterpret_cast<volatile uint32_t *>(smem + S::ABORT);
     const uint32_t tid = threadIdx.x, warp = __shfl_sync(FULL, tid / 32u, 0), lane = tid % 32u;
-    uint32_t rank;
-    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
-    const uint32_t pair = blockIdx.x / 2u, pairs = gridDim.x / 2u;
+    uint32_t in_cluster;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(in_cluster));
+    const uint32_t rank = in_cluster & 1u, first = in_cluster & ~1u, share = in_cluster / 2u;
+    const uint32_t pair = blockIdx.x / (2u * a.shares), pairs = gridDim.x / (2u * a.shares);  // (clusters, with shares)
+    const uint32_t stages = a.stages, stage = A_STAGE + a.tile_tokens / 2u * BLOCK_BYTES;
+    const uint32_t from_step = share * a.blocks / a.shares, to_step = (share + 1u) * a.blocks / a.shares;
     const uint32_t output_tiles = (a.outputs + S::TILE - 1u) / S::TILE, tiles = output_tiles * a.token_tiles;
 
     if (tid == 0) {
-        for (uint32_t s = 0; s < S::STAGES; ++s) {
+        for (uint32_t s = 0; s < S::MOST_STAGES; ++s) {
             mbar_init(base + S::FULL_BARS + 8 * s, 1);
             mbar_init(base + S::EMPTY + 8 * s, 1);
         }
@@ -667,27 +701,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(320, 1) linear_many_
 
     if (warp == 0u) {
         if (lane == 0u) {
-            uint32_t i = 0;  // steps so far
+            uint32_t i = 0, s = 0, phase = 0;  // steps so far; of the ring
             bool gave_up = false;
             for (uint32_t tile = pair; tile < tiles && !gave_up; tile += pairs) {
                 const int32_t output0 = (int32_t)(tile / a.token_tiles * S::TILE + rank * TILE_M);
                 const int32_t token0 = (int32_t)(tile % a.token_tiles * a.tile_tokens + rank * (a.tile_tokens / 2u));
-                for (uint32_t k = 0; k < a.blocks; ++k, ++i) {
-                    const uint32_t s = i % S::STAGES;
-                    if (mbar_wait(base + S::EMPTY + 8 * s, (i / S::STAGES & 1u) ^ 1u, abort_word, a.wait_ns)) {
+                for (uint32_t k = from_step; k < to_step; ++k, ++i) {
+                    if (mbar_wait(base + S::EMPTY + 8 * s, phase ^ 1u, abort_word, a.wait_ns)) {
                         gave_up = true;
                         break;
                     }
-                    const uint32_t bar = base + S::FULL_BARS + 8 * s, to = base + s * S::STAGE;
+                    const uint32_t bar = base + S::FULL_BARS + 8 * s, to = base + s * stage;
+                    s = s + 1u == stages ? 0u : s + 1u;
+                    phase ^= s == 0u;
                     const int32_t x = (int32_t)(k * (E4M3 ? BLOCK_BYTES : BLOCK_BYTES / 2u));
-                    if (i == a.lost_stage && pair == 0u && rank == 0u) {
+                    if (i == a.lost_stage && blockIdx.x == 0u) {
                         continue;  // (test hook: the stage never fills)
                     }
                     if (rank == 0u) {
                         mbar_expect_tx(bar, 2u * A_STAGE + a.tile_tokens * BLOCK_BYTES);
                     }
-                    tma_load_2d_pair(to, &a.w_map, at_rank(bar, 0), x, output0);
-                    tma_load_2d_pair(to + A_STAGE, &a.a_map, at_rank(bar, 0), x, token0);
+                    tma_load_2d_pair(to, &a.w_map, at_rank(bar, first), x, output0);
+                    tma_load_2d_pair(to + A_STAGE, &a.a_map, at_rank(bar, first), x, token0);
                 }
             }
             if (gave_up) {
@@ -701,41 +736,42 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(320, 1) linear_many_
     } else if (warp == 1u && rank == 0u) {
         const bool leader = elect_one();
         const uint32_t idesc = product_desc<E4M3>(2u * TILE_M, a.tile_tokens);
-        uint32_t i = 0, turn = 0;
+        uint32_t s = 0, phase = 0, turn = 0;
         bool gave_up = false;
         for (uint32_t tile = pair; tile < tiles && !gave_up; tile += pairs, ++turn) {
             const uint32_t b = turn % S::ACCS;
             if (warp_wait(base + S::ACC_EMPTY + 8 * b, (turn / S::ACCS & 1u) ^ 1u, abort_word, a.wait_ns)) {
                 break;
             }
-            for (uint32_t k = 0; k < a.blocks; ++k, ++i) {
-                const uint32_t s = i % S::STAGES;
-                if (warp_wait(base + S::FULL_BARS + 8 * s, i / S::STAGES & 1u, abort_word, a.wait_ns)) {
+            for (uint32_t k = from_step; k < to_step; ++k) {
+                if (warp_wait(base + S::FULL_BARS + 8 * s, phase, abort_word, a.wait_ns)) {
                     gave_up = true;
                     break;
                 }
                 tc_fence_after();
                 if (leader) {
-                    const uint64_t adesc = operand_desc(base + s * S::STAGE), bdesc = operand_desc(base + s * S::STAGE + A_STAGE);
+                    const uint64_t adesc = operand_desc(base + s * stage), bdesc = operand_desc(base + s * stage + A_STAGE);
 #pragma unroll
                     for (uint32_t q = 0; q < 4u; ++q) {
-                        mma_ss_pair<E4M3>(tmem + b * S::TILE, adesc + 2u * q, bdesc + 2u * q, idesc, k > 0u || q > 0u);
+                        mma_ss_pair<E4M3>(tmem + b * S::TILE, adesc + 2u * q, bdesc + 2u * q, idesc, k > from_step || q > 0u);
                     }
-                    mma_commit_pair(base + S::EMPTY + 8 * s);
+                    mma_commit_pair(base + S::EMPTY + 8 * s, first);
                 }
                 __syncwarp();
+                s = s + 1u == stages ? 0u : s + 1u;
+                phase ^= s == 0u;
             }
             if (leader && !gave_up) {
-                mma_commit_pair(base + S::ACC_FULL + 8 * b);
+                mma_commit_pair(base + S::ACC_FULL + 8 * b, first);
             }
             __syncwarp();
         }
         if (leader) {
-            mma_commit_pair(base + S::FINAL);
+            mma_commit_pair(base + S::FINAL, first);
             mbar_drain(base + S::FINAL, 0u, a.wait_ns);  // (nothing is freed under a multiply, on any way out)
         }
         __syncwarp();
-    } else if (warp >= 2u) {
+    } else if (warp >= 2u && a.shares == 1u) {
         const uint32_t quad = warp % 4u, half = (warp - 2u) / 4u;
         uint32_t turn = 0, loaded = 0;  // tiles; residuals asked for
         for (uint32_t tile = pair; tile < tiles; tile += pairs, ++turn) {
@@ -745,6 +781,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(320, 1) linear_many_
             const uint32_t live = token0 < a.tokens ? min(tokens, a.tokens - token0) : 0u;
             const uint32_t from = tmem + (quad * 32u << 16) + b * S::TILE + half * tokens;
             const Output o = output_of(a, n);
+            const TokenScales scales(a, token0, live);
             if (a.copies) {
                 const uint32_t w = warp - 2u, mine = base + S::OUT + w * S::WARP_TILE + lane * 2u, bar = base + S::RESIDUAL + 8 * w;
                 const bool any = live > 0u && n - lane < a.outputs;
@@ -783,7 +820,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(320, 1) linear_many_
                     for (uint32_t j = 0; j < 16u; ++j) {
                         v[j] = __uint_as_float(q[j]);
                     }
-                    finish_sums(a, o, token0 + c, live - c, v, r);
+                    finish_sums(a, o, scales, c, v, r);
 #pragma unroll
                     for (uint32_t j = 0; j < 16u; ++j) {
                         asm volatile("st.shared.u16 [%0], %1;" ::"r"(mine + (c + j) * 64u), "h"(__bfloat16_as_ushort(__float2bfloat16_rn(v[j])))
@@ -815,7 +852,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(320, 1) linear_many_
                     for (uint32_t j = 0; j < 16u; ++j) {
                         v[j] = __uint_as_float(q[j]);
                     }
-                    finish(a, o, token0 + c, n, live - c, v, r);
+                    finish(a, o, scales, c, token0 + c, n, live - c, v, r);
 #pragma unroll
                     for (uint32_t j = 0; j < 16u; ++j) {
                         r[j] = next[j];
@@ -826,7 +863,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(320, 1) linear_many_
             __syncwarp();
             if (lane == 0u) {
                 asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
-                                 at_rank(base + S::ACC_EMPTY + 8 * b, 0))
+                                 at_rank(base + S::ACC_EMPTY + 8 * b, first))
                              : "memory");
             }
         }
@@ -836,6 +873,68 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(320, 1) linear_many_
             asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
             if (*abort_word && loaded > 0u) {
                 mbar_drain(base + S::RESIDUAL + 8 * (warp - 2u), (loaded - 1u) & 1u, a.wait_ns);
+            }
+        }
+        __syncwarp();
+    }
+    if (a.shares > 1u) {
+        // One tile a cluster: every pair has multiplied its share of the columns for all of the tile's tokens; it
+        // gets the others' sums of its part of the tokens, adds them up in the order of the shares, and
+        // finishes them. The sums lie over the stages, which nobody needs by then.
+        const uint32_t quad = warp % 4u, half = (warp - 2u) / 4u, row = quad * 32u + lane;
+        const uint32_t n = pair / a.token_tiles * S::TILE + rank * TILE_M + row;
+        const uint32_t per = a.tile_tokens / a.shares;
+        const auto part_at = [&](uint32_t from, uint32_t c) { return base + ((from * (per / 4u) + c / 4u) * TILE_M + row) * 16u; };
+        const uint32_t begin = half * (per / 2u), token0 = pair % a.token_tiles * a.tile_tokens;
+        const uint32_t mine = token0 + share * per + begin;  // this warp's tokens
+        const uint32_t live = mine < a.tokens ? min(per / 2u, a.tokens - mine) : 0u;
+        Output o = {1.0f, 0.0f, false};
+        const TokenScales scales(a, mine, warp >= 2u ? live : 0u);
+        float r[8];
+        bool there = false;
+        if (warp >= 2u) {
+            o = output_of(a, n);
+            residuals_of(a, o, mine, n, live, r);
+            there = !warp_wait(base + S::ACC_FULL, 0u, abort_word, a.wait_ns);
+        }
+        __syncwarp();
+        cluster_arrive();
+        cluster_wait();
+        if (there) {
+            tc_fence_after();
+            for (uint32_t c = half * 16u; c < a.tile_tokens; c += 32u) {
+                uint32_t q[16];
+                tmem_ld16(tmem + (quad * 32u << 16) + c, q);
+                tmem_ld_wait();
+#pragma unroll
+                for (uint32_t j = 0; j < 16u; j += 4u) {
+                    const uint32_t to = (c + j) / per;
+                    asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
+                                     at_rank(part_at(share, c + j - to * per), 2u * to + rank)),
+                                 "r"(q[j]), "r"(q[j + 1u]), "r"(q[j + 2u]), "r"(q[j + 3u])
+                                 : "memory");
+                }
+            }
+        }
+        __syncwarp();
+        cluster_arrive();
+        cluster_wait();
+        if (there) {
+            for (uint32_t c = 0; c < live; c += 8u) {
+                float v[8] = {}, next[8];
+                residuals_of(a, o, mine + c + 8u, n, live > c + 8u ? live - c - 8u : 0u, next);
+                for (uint32_t k = 0; k < a.shares; ++k) {
+#pragma unroll
+                    for (uint32_t j = 0; j < 8u; j += 4u) {
+                        const float4 p = *reinterpret_cast<const float4 *>(smem + (part_at(k, begin + c + j) - base));
+                        v[j] += p.x, v[j + 1u] += p.y, v[j + 2u] += p.z, v[j + 3u] += p.w;
+                    }
+                }
+                finish(a, o, scales, c, mine + c, n, live - c, v, r);
+#pragma unroll
+                for (uint32_t j = 0; j < 8u; ++j) {
+                    r[j] = next[j];
+                }
             }
         }
         __syncwarp();
@@ -867,12 +966,23 @@ cudaError_t set_up(Kernel kernel, uint32_t bytes, std::atomic<uint64_t> &ready) 
 }
 
 template <uint32_t N, bool E4M3>
-cudaError_t launch_few(const LinearArgs &a, uint32_t blocks, uint32_t shares, cudaStream_t stream) {
+cudaError_t launch_few(const LinearArgs &a, uint64_t tiles, uint64_t sms, cudaStream_t stream) {
     static std::atomic<uint64_t> ready{0};
     const cudaError_t e = set_up(linear_few_kernel<N, E4M3>, Few<N>::BYTES, ready);
     if (e != cudaSuccess) {
         return e;
     }
+    // Shares of the columns: as many blocks as there are SMs, of four steps at least, of 64 tokens and bf16 eight
+    // (40 x 2048 x 2048: bf16, eight shares of four 8.8 us, four of eight 7.9; e4m3, four of four 6.3, two of eight
+    // 7.3); up to 32 tokens two on an SM, of eight (24 x 4096 x
+    // 4096: e4m3, four shares of eight steps 7.7 us, eight of four 8.2; bf16, of sixteen 10.6, of eight 9.4;
+    // 64 tokens on one block an SM 12.7 us, on two 14.1).
+    uint32_t shares = 8u;
+    while (shares > 1u && (tiles * shares > sms * (N <= 32u ? 2u : 1u) ||
+                           a.blocks < (tiles * shares > sms || (N > 32u && !E4M3) ? 8u : 4u) * shares)) {
+        shares /= 2u;
+    }
+    const uint32_t blocks = (uint32_t)std::min<uint64_t>(tiles, sms * 2u) * shares;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(blocks, 1, 1);
     cfg.blockDim = dim3(Few<N>::THREADS, 1, 1);
@@ -890,32 +1000,74 @@ cudaError_t launch_few(const LinearArgs &a, uint32_t blocks, uint32_t shares, cu
     return cudaLaunchKernelEx(&cfg, linear_few_kernel<N, E4M3>, a);
 }
 
+// How many clusters of 1 << i pairs run at once, asked once for a device. Not all SMs of a part of it fit into
+// clusters: 74, 33 and 15 of 148 SMs. One tile more than that waits for all the others (300 x 4096 x 2048, sixteen
+// tiles: four shares 25.8 us, two 14.8).
 template <bool E4M3>
-cudaError_t launch_many(const LinearArgs &a, uint32_t pairs, cudaStream_t stream) {
+cudaError_t clusters_at_once(uint64_t (&most)[3]) {
+    static std::atomic<uint64_t> ready{0};
+    static std::atomic<uint32_t> known[64][3] = {};  // (plus one: 0 is not known)
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    for (uint32_t i = 0; e == cudaSuccess && i < 3u; ++i) {
+        std::atomic<uint32_t> &mine = known[device & 63][i];
+        uint32_t seen = mine.load(std::memory_order_relaxed);
+        if (seen == 0u) {
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(2u << i, 1, 1);
+            cfg.blockDim = dim3(Many::THREADS, 1, 1);
+            cfg.dynamicSmemBytes = Many::BYTES;
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = 2u << i;
+            attr[0].val.clusterDim.y = 1;
+            attr[0].val.clusterDim.z = 1;
+            cfg.attrs = attr;
+            cfg.numAttrs = 1;
+            int found = 0;
+            e = set_up(linear_many_kernel<E4M3>, Many::BYTES, ready);
+            if (e == cudaSuccess) {
+                e = cudaOccupancyMaxActiveClusters(&found, linear_many_kernel<E4M3>, &cfg);
+            }
+            seen = (uint32_t)found + 1u;
+            if (e == cudaSuccess) {
+                mine.store(seen, std::memory_order_relaxed);
+            }
+        }
+        most[i] = seen - 1u;
+    }
+    return e;
+}
+
+template <bool E4M3>
+cudaError_t launch_many(const LinearArgs &a, uint32_t clusters, cudaStream_t stream) {
     static std::atomic<uint64_t> ready{0};
     const cudaError_t e = set_up(linear_many_kernel<E4M3>, Many::BYTES, ready);
     if (e != cudaSuccess) {
         return e;
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(2u * pairs, 1, 1);
+    cfg.gridDim = dim3(2u * a.shares * clusters, 1, 1);
     cfg.blockDim = dim3(Many::THREADS, 1, 1);
     cfg.dynamicSmemBytes = Many::BYTES;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = 2u * a.shares;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     return cudaLaunchKernelEx(&cfg, linear_many_kernel<E4M3>, a);
 }
 
 template <bool E4M3>
-cudaError_t few_by_tokens(const LinearArgs &a, uint32_t n, uint32_t blocks, uint32_t shares, cudaStream_t stream) {
-    return n == 16u   ? launch_few<16, E4M3>(a, blocks, shares, stream)
-           : n == 32u ? launch_few<32, E4M3>(a, blocks, shares, stream)
-           : n == 64u ? launch_few<64, E4M3>(a, blocks, shares, stream)
-                      : launch_few<128, E4M3>(a, blocks, shares, stream);
+cudaError_t few_by_tokens(const LinearArgs &a, uint32_t n, uint64_t tiles, uint64_t sms, cudaStream_t stream) {
+    return n == 16u   ? launch_few<16, E4M3>(a, tiles, sms, stream)
+           : n == 32u ? launch_few<32, E4M3>(a, tiles, sms, stream)
+                      : launch_few<64, E4M3>(a, tiles, sms, stream);
 }
 
 bool encode_rows(CUtensorMap *map, const void *p, uint64_t ld, uint32_t rows, uint32_t columns, uint32_t dtype,
@@ -1005,23 +1157,37 @@ extern "C" int32_t lily_linear(lily_sampler_t *h, void *stream_, const lily_line
     h->lost_stage = 0xFFFFFFFFu;  // one launch only
 
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-    // Pairs of blocks above 128 tokens, unless the tiles would leave half of the SMs idle and the columns are long
-    // enough to be shared: 64 steps. Pairs do not share columns (pairs, and single blocks that share, in us:
-    // 256 x 2048 x 11000 19 and 24, 640 x 4096 x 4096 24 and 37, 1024 x 1024 x 1024 8.6 and 10.7; the other
-    // way 256 x 4096 x 4096 22 and 17, 300 x 8192 x 2048 38 and 23, 1024 x 4096 x 1024 21 and 16).
     const uint64_t sms = (uint32_t)h->sm_count;
-    const uint64_t singles = (g.tokens + 127ull) / 128u * ((g.outputs + TILE_M - 1ull) / TILE_M);
-    if (g.tokens > 128u && (singles * 2u > sms || a.blocks < 64u)) {
-        // The tile's tokens: the shortest way for the busiest pair. A smaller tile costs little less than one of
-        // 256 tokens (4099 x 4096 x 4096: five of 192 in turn 107 us, four of 256 96 to 98; 8192 x 8192 x 4096:
-        // 544 and 409): what is read for a tile, the weights above all, stays.
-        const uint64_t pairs = sms / 2u, output_tiles = (g.outputs + Many::TILE - 1ull) / Many::TILE;
+    if (g.tokens > 64u) {
+        const auto rows16 = [&](const void *p, uint64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16u == 0u && ld * 2u % 16u == 0u; };
+        // (A copy out of shared memory writes whole 16 bytes: rows of 1003 outputs had zeroes behind them.)
+        const bool copies = !a.out_f32 && g.outputs % 8u == 0u && rows16(g.out, g.out_ld) &&
+                            (g.residual == nullptr || rows16(g.residual, g.residual_ld));
+        // The tile's tokens and the shares of its columns, by the time of the busiest pair, in units of which 1900
+        // are a microsecond. A step takes the longest of its multiplies (256 tokens 0.27 us), of what all pairs
+        // read (256 + t rows of 128 bytes each, 11.5 TB/s together), and of a copy's way (1.35 us) by the stages there
+        // are. A tile's end costs by its tokens (16 ns each), joining shares by the sums that are sent (two of 256 tokens 5 us).
+        uint64_t most[3] = {};
+        CU(h, e4m3 ? clusters_at_once<true>(most) : clusters_at_once<false>(most));
+        const uint64_t pairs = most[0], output_tiles = (g.outputs + Many::TILE - 1ull) / Many::TILE;
+        if (pairs == 0u) {
+            return fail(h, LILY_ERR_CUDA, "the device has no room for a pair of blocks");
+        }
         uint64_t best = ~0ull;
         for (uint32_t t = Many::TILE; t >= 64u; t -= 32u) {
-            const uint64_t tiles = (g.tokens + t - 1u) / t * output_tiles, cost = (tiles + pairs - 1u) / pairs * (t + 320u);
-            if (cost < best) {
-                best = cost;
-                a.tile_tokens = t;
+            const uint64_t tiles = (g.tokens + t - 1u) / t * output_tiles;
+            for (uint32_t i = 0, shares = 1u; i < 3u; ++i, shares *= 2u) {
+                if (shares > 1u && (tiles > most[i] || a.blocks < 8u * shares || t % (16u * shares) != 0u)) {
+                    continue;
+                }
+                const uint32_t stages = Many::stages_of(t, copies && shares == 1u);
+                const uint64_t steps = (tiles + pairs - 1u) / pairs * ((a.blocks + shares - 1u) / shares);
+                const uint64_t step = std::max<uint64_t>({2u * t, (256u + t) * std::min(tiles * shares, pairs) * 2u / 95u, 2565u / stages});
+                const uint64_t cost = steps * step + t / shares * 31u + (shares > 1u ? t * (shares - 1u) / shares * 70u + 1000u : 0u);
+                if (cost < best) {
+                    best = cost;
+                    a.tile_tokens = t, a.shares = shares, a.stages = stages, a.copies = copies && shares == 1u;
+                }
             }
         }
         a.token_tiles = (g.tokens + a.tile_tokens - 1u) / a.tile_tokens;
@@ -1029,37 +1195,22 @@ extern "C" int32_t lily_linear(lily_sampler_t *h, void *stream_, const lily_line
         if (tiles > 0x7FFFFFFFull) {
             return fail(h, LILY_ERR_CAPACITY, "more tiles than a launch takes");
         }
-        const auto rows16 = [&](const void *p, uint64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16u == 0u && ld * 2u % 16u == 0u; };
-        // (A copy out of shared memory writes whole 16 bytes: rows of 1003 outputs had zeroes behind them.)
-        a.copies = !a.out_f32 && g.outputs % 8u == 0u && rows16(g.out, g.out_ld) && (g.residual == nullptr || rows16(g.residual, g.residual_ld));
         if (!encode_rows(&a.w_map, g.weight, g.weight_ld, g.outputs, g.columns, g.dtype, TILE_M) ||
             !encode_rows(&a.a_map, g.a, g.a_ld, g.tokens, g.columns, g.dtype, a.tile_tokens / 2u) ||
             (a.copies && (!encode_outs(&a.out_map, g.out, g.out_ld, g, a.tile_tokens / 2u) ||
                           (g.residual != nullptr && !encode_outs(&a.residual_map, g.residual, g.residual_ld, g, a.tile_tokens / 2u))))) {
             return fail(h, LILY_ERR_CUDA, "cuTensorMapEncodeTiled refused a, weight, out or residual");
         }
-        const uint32_t used = (uint32_t)std::min(tiles, pairs);
+        const uint32_t used = (uint32_t)std::min(tiles, pairs);  // (with shares, fewer tiles than pairs)
         CU(h, e4m3 ? launch_many<true>(a, used, stream) : launch_many<false>(a, used, stream));
         return LILY_OK;
     }
-    const uint32_t n = g.tokens <= 16u ? 16u : g.tokens <= 32u ? 32u : g.tokens <= 64u ? 64u : 128u;
+    const uint32_t n = g.tokens <= 16u ? 16u : g.tokens <= 32u ? 32u : 64u;
     if (!encode_rows(&a.w_map, g.weight, g.weight_ld, g.outputs, g.columns, g.dtype, TILE_M) ||
         !encode_rows(&a.a_map, g.a, g.a_ld, g.tokens, g.columns, g.dtype, n)) {
         return fail(h, LILY_ERR_CUDA, "cuTensorMapEncodeTiled refused a or weight");
     }
-    a.token_tiles = (g.tokens + n - 1u) / n;
-    const uint64_t tiles = (uint64_t)a.token_tiles * ((g.outputs + TILE_M - 1u) / TILE_M);
-    if (tiles > 0x7FFFFFFFull) {
-        return fail(h, LILY_ERR_CAPACITY, "more tiles than a launch takes");
-    }
-    // Shares of the columns: as many blocks as there are SMs, of four steps at least; up to 32 tokens two on
-    // an SM, of eight (24 x 4096 x 4096: e4m3, four shares of eight steps 7.7 us, eight of four 8.2; bf16, of
-    // sixteen 10.6, of eight 9.4; 64 tokens on one block an SM 12.7 us, on two 14.1).
-    uint32_t shares = 8u;
-    while (shares > 1u && (tiles * shares > sms * (n <= 32u ? 2u : 1u) || a.blocks < (tiles * shares > sms ? 8u : 4u) * shares)) {
-        shares /= 2u;
-    }
-    const uint32_t blocks = (uint32_t)std::min<uint64_t>(tiles, sms * (n <= 64u ? 2u : 1u)) * shares;
-    CU(h, e4m3 ? few_by_tokens<true>(a, n, blocks, shares, stream) : few_by_tokens<false>(a, n, blocks, shares, stream));
+    const uint64_t tiles = (g.outputs + TILE_M - 1ull) / TILE_M;
+    CU(h, e4m3 ? few_by_tokens<true>(a, n, tiles, sms, stream) : few_by_tokens<false>(a, n, tiles, sms, stream));
     return LILY_OK;
 }

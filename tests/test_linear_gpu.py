@@ -69,7 +69,8 @@ def _check(torch, out, a, w, kw, bias=None, act="none", residual=None):
 
 SIZES = [(1, 2048, 2048), (1, 16, 1), (1, 8, 130), (2, 100, 300), (7, 1000, 129), (16, 4096, 512), (17, 520, 257),
          (24, 4096, 4096), (32, 64, 128), (33, 192, 1000), (64, 2048, 777), (65, 512, 384), (128, 1024, 1024),
-         (129, 320, 640), (200, 2048, 1000), (257, 640, 515), (512, 1024, 2048), (700, 96, 4096), (2049, 512, 1025)]
+         (129, 320, 640), (200, 2048, 1000), (257, 640, 515), (512, 1024, 2048), (700, 96, 4096), (2049, 512, 1025),
+         (150, 4096, 300), (300, 2064, 520), (513, 4096, 513), (1024, 2048, 1024), (190, 8192, 2050)]
 
 
 @pytest.mark.parametrize("tokens,columns,outputs", SIZES)
@@ -154,6 +155,25 @@ def test_rows_on_boundaries_and_off_them_give_the_same(cuda, lily):
         scratch.linear(a, w, out, activation=act, residual=residual)
         scratch.linear(a, w, odd, activation=act, residual=odd_residual)
         assert torch.equal(out, odd)
+
+
+def test_lost_copy_among_shares(cuda, lily):
+    """Few tiles of long columns, which several blocks share: one of them gives up, all of them end."""
+    torch = cuda
+    g = torch.Generator(device="cuda").manual_seed(23)
+    scratch = _handle(lily)
+    for tokens, outputs in ((70, 200), (300, 256), (300, 1024), (500, 2048)):
+        a, w, kw = _inputs(torch, g, tokens, 4096, outputs, "bf16")
+        out = torch.empty((tokens, outputs), device="cuda")
+        for stage in (0, 6):
+            scratch.set_wait_limit(20_000_000)
+            scratch.inject_lost_copy(stage)
+            scratch.linear(a, w, out)
+            assert scratch.status() == lily.ERR_TIMEOUT
+            scratch.set_wait_limit(0)
+            scratch.linear(a, w, out)
+            assert scratch.status() == lily.OK
+            _check(torch, out, a, w, kw)
 
 
 def test_lost_copy_with_a_residual(cuda, lily):
