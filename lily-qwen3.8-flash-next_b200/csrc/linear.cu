@@ -29,7 +29,7 @@ constexpr uint32_t A_STAGE = TILE_M * BLOCK_BYTES;
 constexpr uint32_t FULL = 0xFFFFFFFFu;
 
 struct LinearArgs {
-    CUtensorMap w_map;  // [outputs, columns], boxes of 128 rows x 128 bytes, 128-byte swizzle
+    CUtensorMap w_map;  // [outputs, columns], boxes of a tile's rows (many tokens: a block's 128) x 128 bytes, 128-byte swizzle
     CUtensorMap a_map;  // [tokens, columns], boxes of a token tile (many tokens: half of one) x 128 bytes
     CUtensorMap out_map, residual_map;  // many tokens, `copies`: bf16 [tokens, outputs], boxes of half a tile x 32 outputs
     const float *a_scales, *w_scales;
@@ -38,11 +38,12 @@ struct LinearArgs {
     uint64_t residual_ld, out_ld;
     uint32_t tokens, outputs;
     uint32_t blocks;        // steps of BLOCK_BYTES in a row
-    uint32_t token_tiles;
+    uint32_t tile_outputs;  // few tokens: of a tile, a multiple of 8
+    uint32_t token_tiles;   // many tokens
     uint32_t tile_tokens;   // many tokens: of a tile, a multiple of 32
     uint32_t copies;        // many tokens: out and residual go through shared memory
     uint32_t shares;        // many tokens: pairs of a cluster that share a tile's columns
-    uint32_t stages;        // many tokens: of the pipeline
+    uint32_t stages;        // of the pipeline
     uint32_t out_f32, bias_f32, activation;
     uint32_t *status_word;
     uint64_t wait_ns;
@@ -238,20 +239,24 @@ __device__ __forceinline__ uint32_t at_rank(uint32_t addr, uint32_t rank) {
 
 // ------------------------------------------------------------------ few tokens --
 //
-// Tiles of 128 outputs x N tokens. Many of them: a block has one after the other, and finishes one while
-// it multiplies the next. Few: a cluster has one, whose columns its blocks share out evenly. Each
+// Up to 64 tokens. Many tiles, of up to 128 outputs x N tokens: a block has one after the other, and finishes one
+// while it multiplies the next; the tile's outputs are as many as give all blocks the same (1 x 4096 x 40000: with
+// 128 for 313 tiles on 296 blocks 60 us, with 72 51: 6.4 TB/s). Few: a cluster has one of 128, whose columns its blocks share out evenly. Each
 // sums its share in tensor memory, then sends every token's column of sums to the block that finishes that
 // token, which adds the shares up in the blocks' order.
+//
+// What bounds it: the weights' stream (16 x 2048 x 151936 94 us, 6.7 TB/s); below about 50 MB of them a launch's
+// fixed costs, 3 us, and a copy's way of a microsecond for as many steps as a block has stages.
 //
 // A block's warps: 0 asks for the copies, 1 issues the multiplies, 2 to 5 are the epilogue.
 template <uint32_t N>
 struct Few {
     static constexpr uint32_t THREADS = 192;
     static constexpr uint32_t B_STAGE = N * BLOCK_BYTES;
-    static constexpr uint32_t STAGE = A_STAGE + B_STAGE;
     static constexpr uint32_t PART_BYTES = N * TILE_M * 4u;
     // Two blocks on an SM.
-    static constexpr uint32_t STAGES = N == 16u ? 5u : 4u;
+    static constexpr uint32_t MOST_STAGES = 10;
+    static constexpr uint32_t RING = (N == 16u ? 5u : 4u) * (A_STAGE + B_STAGE);  // bytes of stages
     // The sums that blocks send one another have a place of their own (a block may send as soon as the
     // other runs), or, where that takes a stage, the stages' (it has to be done with its columns).
     static constexpr bool OVER_STAGES = N >= 64u;
@@ -259,17 +264,22 @@ struct Few {
     // tile is finished while the block's next one is multiplied.
     static constexpr uint32_t ACCS = 2, SETS = 2;
     static constexpr uint32_t COLS = SETS * ACCS * N;
-    static constexpr uint32_t PART = OVER_STAGES ? 0u : STAGES * STAGE;
-    static constexpr uint32_t BARS = STAGES * STAGE + (OVER_STAGES ? 0u : PART_BYTES);
-    static_assert(PART_BYTES <= STAGES * STAGE, "room for the sums");
-    static constexpr uint32_t EMPTY = BARS + 8u * STAGES;
-    static constexpr uint32_t ACC_FULL = EMPTY + 8u * STAGES;
+    static constexpr uint32_t PART = OVER_STAGES ? 0u : RING;
+    static constexpr uint32_t BARS = RING + (OVER_STAGES ? 0u : PART_BYTES);
+    static_assert(PART_BYTES <= RING, "room for the sums");
+    static constexpr uint32_t EMPTY = BARS + 8u * MOST_STAGES;
+    static constexpr uint32_t ACC_FULL = EMPTY + 8u * MOST_STAGES;
     static constexpr uint32_t ACC_EMPTY = ACC_FULL + 8u * SETS;
     static constexpr uint32_t FINAL = ACC_EMPTY + 8u * SETS;
     static constexpr uint32_t TMEM_ADDR = FINAL + 8u;
     static constexpr uint32_t ABORT = TMEM_ADDR + 4u;
     static constexpr uint32_t BYTES = ABORT + 4u + 1024u;
     static_assert(BYTES <= 227u * 1024u && BYTES > 76u * 1024u, "at most two blocks on an SM");
+    // (A multiply reads 128 rows of every stage, the last one's too: they lie in the ring.)
+    static constexpr uint32_t stages_of(uint32_t outputs) {
+        const uint32_t stage = outputs * BLOCK_BYTES + B_STAGE, n = (RING - A_STAGE) / stage + 1u, all = RING / stage;
+        return n < all ? (n < MOST_STAGES ? n : MOST_STAGES) : all < MOST_STAGES ? all : MOST_STAGES;
+    }
     static_assert(COLS >= 32u && COLS <= 256u && (COLS & (COLS - 1u)) == 0u, "tensor memory of two blocks on an SM");
 };
 
@@ -285,13 +295,14 @@ __global__ void __launch_bounds__(192) linear_few_kernel(const __grid_constant__
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(shares));
     const uint32_t tile0 = blockIdx.x / shares, stride = gridDim.x / shares;
-    const uint32_t tiles = (a.outputs + TILE_M - 1u) / TILE_M;
-    const auto output_tile = [&](uint32_t tile) { return tile * TILE_M; };
+    const uint32_t tiles = (a.outputs + a.tile_outputs - 1u) / a.tile_outputs;
+    const uint32_t stages = a.stages, a_stage = a.tile_outputs * BLOCK_BYTES, stage = a_stage + S::B_STAGE;
+    const auto output_tile = [&](uint32_t tile) { return tile * a.tile_outputs; };
     const uint32_t block0 = (uint32_t)((uint64_t)a.blocks * rank / shares);
     const uint32_t steps = (uint32_t)((uint64_t)a.blocks * (rank + 1u) / shares) - block0;
 
     if (tid == 0) {
-        for (uint32_t s = 0; s < S::STAGES; ++s) {
+        for (uint32_t s = 0; s < S::MOST_STAGES; ++s) {
             mbar_init(base + S::BARS + 8 * s, 1);
             mbar_init(base + S::EMPTY + 8 * s, 1);
         }
@@ -323,29 +334,30 @@ __global__ void __launch_bounds__(192) linear_few_kernel(const __grid_constant__
 
     if (warp == 0u) {
         if (lane == 0u) {
-            uint32_t asked = 0, parity = 0, i = 0;
+            uint32_t asked = 0, parity = 0, i = 0, s = 0, use = 0;
             for (uint32_t tile = tile0; tile < tiles; tile += stride) {
                 const int32_t output0 = (int32_t)output_tile(tile);
                 for (uint32_t k = 0; k < steps; ++k, ++i) {
-                    const uint32_t s = i % S::STAGES, use = i / S::STAGES;
-                    if (mbar_wait(base + S::EMPTY + 8 * s, (use & 1u) ^ 1u, abort_word, a.wait_ns)) {
+                    if (mbar_wait(base + S::EMPTY + 8 * s, use ^ 1u, abort_word, a.wait_ns)) {
                         tile = tiles - stride;  // (the last one)
                         break;
                     }
-                    const uint32_t bar = base + S::BARS + 8 * s, to = base + s * S::STAGE;
+                    const uint32_t at = s, bar = base + S::BARS + 8 * s, to = base + s * stage, phase = use;
+                    s = s + 1u == stages ? 0u : s + 1u;
+                    use ^= s == 0u;
                     const int32_t x = (int32_t)((block0 + k) * (E4M3 ? BLOCK_BYTES : BLOCK_BYTES / 2u));
                     if (i == a.lost_stage && blockIdx.x == 0u) {
                         continue;  // (test hook: the stage never fills)
                     }
-                    asked |= 1u << s;
-                    parity = (parity & ~(1u << s)) | (use & 1u) << s;
-                    mbar_expect_tx(bar, S::STAGE);
+                    asked |= 1u << at;
+                    parity = (parity & ~(1u << at)) | phase << at;
+                    mbar_expect_tx(bar, stage);
                     tma_load_2d(to, &a.w_map, bar, x, output0);
-                    tma_load_2d(to + A_STAGE, &a.a_map, bar, x, 0);
+                    tma_load_2d(to + a_stage, &a.a_map, bar, x, 0);
                 }
             }
             if (*abort_word) {  // the copies asked for land in this block's shared memory: it stays until they have
-                for (uint32_t s = 0; s < S::STAGES; ++s) {
+                for (s = 0; s < stages; ++s) {
                     if (asked >> s & 1u) {
                         mbar_drain(base + S::BARS + 8 * s, parity >> s & 1u, a.wait_ns);
                     }
@@ -356,22 +368,21 @@ __global__ void __launch_bounds__(192) linear_few_kernel(const __grid_constant__
     } else if (warp == 1u) {
         const bool leader = elect_one();
         const uint32_t idesc = product_desc<E4M3>(TILE_M, N);
-        uint32_t i = 0, turn = 0;
+        uint32_t s = 0, use = 0, turn = 0;
         bool gave_up = false;
         for (uint32_t tile = tile0; tile < tiles && !gave_up; tile += stride, ++turn) {
             const uint32_t b = turn % S::SETS;
             if (warp_wait(base + S::ACC_EMPTY + 8 * b, (turn / S::SETS & 1u) ^ 1u, abort_word, a.wait_ns)) {
                 break;
             }
-            for (uint32_t k = 0; k < steps; ++k, ++i) {
-                const uint32_t s = i % S::STAGES;
-                if (warp_wait(base + S::BARS + 8 * s, i / S::STAGES & 1u, abort_word, a.wait_ns)) {
+            for (uint32_t k = 0; k < steps; ++k) {
+                if (warp_wait(base + S::BARS + 8 * s, use, abort_word, a.wait_ns)) {
                     gave_up = true;
                     break;
                 }
                 tc_fence_after();
                 if (leader) {
-                    const uint64_t adesc = operand_desc(base + s * S::STAGE), bdesc = operand_desc(base + s * S::STAGE + A_STAGE);
+                    const uint64_t adesc = operand_desc(base + s * stage), bdesc = operand_desc(base + s * stage + a_stage);
 #pragma unroll
                     for (uint32_t q = 0; q < 4u; ++q) {
                         mma_ss<E4M3>(tmem + (b * S::ACCS + k % S::ACCS) * N, adesc + 2u * q, bdesc + 2u * q, idesc, k >= S::ACCS || q > 0u);
@@ -379,6 +390,8 @@ __global__ void __launch_bounds__(192) linear_few_kernel(const __grid_constant__
                     mma_commit(base + S::EMPTY + 8 * s);
                 }
                 __syncwarp();
+                s = s + 1u == stages ? 0u : s + 1u;
+                use ^= s == 0u;
             }
             if (leader && !gave_up) {
                 mma_commit(base + S::ACC_FULL + 8 * b);
@@ -422,7 +435,8 @@ __global__ void __launch_bounds__(192) linear_few_kernel(const __grid_constant__
         uint32_t turn = 0;
         for (uint32_t tile = tile0; warp >= 2u && tile < tiles; tile += stride, ++turn) {
             const uint32_t b = turn % S::SETS, n = output_tile(tile) + row, live = a.tokens;
-            const Output o = output_of(a, n);
+            Output o = output_of(a, n);
+            o.live = o.live && row < a.tile_outputs;  // (the other rows multiply what lies in the stage)
             const TokenScales scales(a, 0u, live);
             float r[16];
             residuals_of(a, o, 0u, n, live, r);  // (asked for a round ahead, here and below)
@@ -966,23 +980,12 @@ cudaError_t set_up(Kernel kernel, uint32_t bytes, std::atomic<uint64_t> &ready) 
 }
 
 template <uint32_t N, bool E4M3>
-cudaError_t launch_few(const LinearArgs &a, uint64_t tiles, uint64_t sms, cudaStream_t stream) {
+cudaError_t launch_few(const LinearArgs &a, uint32_t blocks, uint32_t shares, cudaStream_t stream) {
     static std::atomic<uint64_t> ready{0};
     const cudaError_t e = set_up(linear_few_kernel<N, E4M3>, Few<N>::BYTES, ready);
     if (e != cudaSuccess) {
         return e;
     }
-    // Shares of the columns: as many blocks as there are SMs, of four steps at least, of 64 tokens and bf16 eight
-    // (40 x 2048 x 2048: bf16, eight shares of four 8.8 us, four of eight 7.9; e4m3, four of four 6.3, two of eight
-    // 7.3); up to 32 tokens two on an SM, of eight (24 x 4096 x
-    // 4096: e4m3, four shares of eight steps 7.7 us, eight of four 8.2; bf16, of sixteen 10.6, of eight 9.4;
-    // 64 tokens on one block an SM 12.7 us, on two 14.1).
-    uint32_t shares = 8u;
-    while (shares > 1u && (tiles * shares > sms * (N <= 32u ? 2u : 1u) ||
-                           a.blocks < (tiles * shares > sms || (N > 32u && !E4M3) ? 8u : 4u) * shares)) {
-        shares /= 2u;
-    }
-    const uint32_t blocks = (uint32_t)std::min<uint64_t>(tiles, sms * 2u) * shares;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(blocks, 1, 1);
     cfg.blockDim = dim3(Few<N>::THREADS, 1, 1);
@@ -1064,10 +1067,10 @@ cudaError_t launch_many(const LinearArgs &a, uint32_t clusters, cudaStream_t str
 }
 
 template <bool E4M3>
-cudaError_t few_by_tokens(const LinearArgs &a, uint32_t n, uint64_t tiles, uint64_t sms, cudaStream_t stream) {
-    return n == 16u   ? launch_few<16, E4M3>(a, tiles, sms, stream)
-           : n == 32u ? launch_few<32, E4M3>(a, tiles, sms, stream)
-                      : launch_few<64, E4M3>(a, tiles, sms, stream);
+cudaError_t few_by_tokens(const LinearArgs &a, uint32_t n, uint32_t blocks, uint32_t shares, cudaStream_t stream) {
+    return n == 16u   ? launch_few<16, E4M3>(a, blocks, shares, stream)
+           : n == 32u ? launch_few<32, E4M3>(a, blocks, shares, stream)
+                      : launch_few<64, E4M3>(a, blocks, shares, stream);
 }
 
 bool encode_rows(CUtensorMap *map, const void *p, uint64_t ld, uint32_t rows, uint32_t columns, uint32_t dtype,
@@ -1206,11 +1209,42 @@ extern "C" int32_t lily_linear(lily_sampler_t *h, void *stream_, const lily_line
         return LILY_OK;
     }
     const uint32_t n = g.tokens <= 16u ? 16u : g.tokens <= 32u ? 32u : 64u;
-    if (!encode_rows(&a.w_map, g.weight, g.weight_ld, g.outputs, g.columns, g.dtype, TILE_M) ||
+    // Shares of the columns: as many blocks as there are SMs, of four steps at least, of 64 tokens and bf16 eight
+    // (40 x 2048 x 2048: bf16, eight shares of four 8.8 us, four of eight 7.9; e4m3, four of four 6.3, two of eight
+    // 7.3); up to 32 tokens two on an SM, of eight (24 x 4096 x 4096: e4m3, four shares of eight steps 7.7 us, eight
+    // of four 8.2; bf16, of sixteen 10.6, of eight 9.4; 64 tokens on one block an SM 12.7 us, on two 14.1).
+    uint64_t tiles = (g.outputs + TILE_M - 1ull) / TILE_M;
+    uint32_t shares = 8u;
+    while (shares > 1u && (tiles * shares > sms * (n <= 32u ? 2u : 1u) ||
+                           a.blocks < (tiles * shares > sms || (n > 32u && !e4m3) ? 8u : 4u) * shares)) {
+        shares /= 2u;
+    }
+    // A tile's outputs, where blocks have tiles of their own: those of which the busiest block is done first. A step
+    // takes the longest of its weights' rows (6.5 TB/s for all blocks together), of these and the tokens', which every
+    // tile reads again (11 TB/s), and of a copy's way (1.35 us) by the stages there are.
+    const auto stages_of = [n](uint32_t outputs) {
+        return n == 16u ? Few<16>::stages_of(outputs) : n == 32u ? Few<32>::stages_of(outputs) : Few<64>::stages_of(outputs);
+    };
+    a.tile_outputs = TILE_M;
+    if (shares == 1u) {
+        uint64_t best = ~0ull;
+        for (uint32_t rows = TILE_M; rows >= 48u; rows -= 8u) {
+            const uint64_t count = (g.outputs + rows - 1ull) / rows, active = std::min(count, 2u * sms);
+            const uint64_t step = std::max<uint64_t>({rows * 10u * active / (2u * sms), (rows + n) * 6u * active / (2u * sms), 2310u / stages_of(rows)});
+            const uint64_t cost = (count + 2u * sms - 1u) / (2u * sms) * step;
+            if (cost < best) {
+                best = cost;
+                a.tile_outputs = rows;
+            }
+        }
+        tiles = (g.outputs + a.tile_outputs - 1ull) / a.tile_outputs;
+    }
+    a.stages = stages_of(a.tile_outputs);
+    if (!encode_rows(&a.w_map, g.weight, g.weight_ld, g.outputs, g.columns, g.dtype, a.tile_outputs) ||
         !encode_rows(&a.a_map, g.a, g.a_ld, g.tokens, g.columns, g.dtype, n)) {
         return fail(h, LILY_ERR_CUDA, "cuTensorMapEncodeTiled refused a or weight");
     }
-    const uint64_t tiles = (g.outputs + TILE_M - 1ull) / TILE_M;
-    CU(h, e4m3 ? few_by_tokens<true>(a, n, tiles, sms, stream) : few_by_tokens<false>(a, n, tiles, sms, stream));
+    const uint32_t blocks = (uint32_t)std::min<uint64_t>(tiles, sms * 2u) * shares;
+    CU(h, e4m3 ? few_by_tokens<true>(a, n, blocks, shares, stream) : few_by_tokens<false>(a, n, blocks, shares, stream));
     return LILY_OK;
 }

@@ -70,7 +70,8 @@ def _check(torch, out, a, w, kw, bias=None, act="none", residual=None):
 SIZES = [(1, 2048, 2048), (1, 16, 1), (1, 8, 130), (2, 100, 300), (7, 1000, 129), (16, 4096, 512), (17, 520, 257),
          (24, 4096, 4096), (32, 64, 128), (33, 192, 1000), (64, 2048, 777), (65, 512, 384), (128, 1024, 1024),
          (129, 320, 640), (200, 2048, 1000), (257, 640, 515), (512, 1024, 2048), (700, 96, 4096), (2049, 512, 1025),
-         (150, 4096, 300), (300, 2064, 520), (513, 4096, 513), (1024, 2048, 1024), (190, 8192, 2050)]
+         (150, 4096, 300), (300, 2064, 520), (513, 4096, 513), (1024, 2048, 1024), (190, 8192, 2050),
+         (37, 256, 50257), (5, 128, 38001), (64, 1024, 11000), (16, 72, 40003), (30, 640, 21001)]
 
 
 @pytest.mark.parametrize("tokens,columns,outputs", SIZES)
@@ -158,11 +159,12 @@ def test_rows_on_boundaries_and_off_them_give_the_same(cuda, lily):
 
 
 def test_lost_copy_among_shares(cuda, lily):
-    """Few tiles of long columns, which several blocks share: one of them gives up, all of them end."""
+    """Few tiles of long columns, which several blocks share: one of them gives up, all of them end. And many
+    tiles in turn."""
     torch = cuda
     g = torch.Generator(device="cuda").manual_seed(23)
     scratch = _handle(lily)
-    for tokens, outputs in ((70, 200), (300, 256), (300, 1024), (500, 2048)):
+    for tokens, outputs in ((70, 200), (300, 256), (300, 1024), (500, 2048), (30, 40000), (64, 11000)):
         a, w, kw = _inputs(torch, g, tokens, 4096, outputs, "bf16")
         out = torch.empty((tokens, outputs), device="cuda")
         for stage in (0, 6):
