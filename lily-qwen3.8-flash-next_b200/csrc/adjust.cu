@@ -11,6 +11,13 @@
 // reads the history again to count them by their numbers: a few thousand counts instead of one for every
 // id. When both are done, the numbered ids, which lie evenly on the threads, are penalised. Blocks have nothing
 // to say to one another, so nothing is kept between calls and no workspace is needed.
+//
+// What bounds it: masks alone are a launch (1 x 151936 2.2 us on the device). 256 x 151936 bf16 to f32 with
+// histories of 32768 ids take 75 us where the bytes are 26: the history's half takes them (three reads of its ids, an
+// atomic in shared memory for each in two of them, scattered logits at the end), and a row is one block's, so
+// 256 of them fill 148 SMs unevenly. Slower there: counts of 16 bits for every id over four slices a row (116 us),
+// the rows' lists pulled by halves of a block (100), tasks in a pipeline (82 to 100), numbers handed out by
+// atomics that return (105).
 #include <cuda_bf16.h>
 
 #include <algorithm>

@@ -5,6 +5,10 @@
 // 8-bit codes, and nothing else of size. One reduction serves both statistics: with u = h * weight,
 // y = u / rms, so the largest |y| is the largest |u| over rms, and the 8-bit codes need no
 // second round through the block.
+//
+// What bounds it: memory from a few hundred tokens on (16384 x 4096 bf16 to codes 72 to 77 us with
+// its residual, 6.5 to 6.1 TB/s; 777 x 5001 f32 8.2 us, out of L2 in part); below, the launch and one way through a block:
+// 1.5 us on the device, 3 through a Python call.
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 
