@@ -761,6 +761,16 @@ extern "C" int32_t lily_adjust_logits(lily_sampler_t *h, void *stream_, const li
         (g.bias_ids != nullptr) != (g.bias_vals != nullptr) || (g.ban_ids != nullptr) != (g.ban_len != nullptr)) {
         return fail(h, LILY_ERR_ARG, "a list needs both its ids and its lengths");
     }
+    for (const void *words : {(const void *)g.history_ids, (const void *)g.history_len, (const void *)g.bias_ids, (const void *)g.bias_vals,
+                              (const void *)g.bias_len, (const void *)g.ban_ids, (const void *)g.ban_len, (const void *)g.mask,
+                              (const void *)g.mask_rows, (const void *)g.out_status}) {
+        if (reinterpret_cast<uintptr_t>(words) % 4u) {
+            return fail(h, LILY_ERR_ARG, "a list, a mask or a status is not aligned to its words");
+        }
+    }
+    if (g.params_on_device && reinterpret_cast<uintptr_t>(g.params) % alignof(lily_sampling_params_t)) {
+        return fail(h, LILY_ERR_ARG, "params are not aligned");
+    }
     if ((uint64_t)g.first_id + h->vocab > 0xFFFFFFFFull) {
         return fail(h, LILY_ERR_ARG, "first_id + vocab overflows an id");
     }

@@ -594,16 +594,19 @@ __global__ void __launch_bounds__(192) linear_few_kernel(const __grid_constant__
 // busy for three quarters of the time, the board's power; below about 1000 tokens the launch, the pipeline's
 // first copies and the last tile's end, 5 us together.
 //
-// A block's warps: 0 asks for the block's copies, 1 issues the pair's multiplies (in the first block
+// A block's warps: 0 and 10 ask for the block's copies in turn (one alone took 0.25 us for a step's two: 300 x 8192 x 2048
+// 23.8 us, with two warps 20.4; three and four give the same), 1 issues the pair's multiplies (in the first block
 // of the pair alone), 2 to 9 are the epilogue, two for each quarter of tensor memory's lanes.
 struct Many {
-    static constexpr uint32_t THREADS = 320;
+    static constexpr uint32_t ASKERS = 2;
+    static constexpr uint32_t THREADS = 288 + 32 * ASKERS;
     static constexpr uint32_t TILE = 256;          // of outputs, and the most of tokens
     static constexpr uint32_t MOST_STAGES = 11;
     static constexpr uint32_t RING = 5u * 2u * A_STAGE;  // bytes of stages: a block's half of the weights, and of the tokens
     static constexpr uint32_t WARP_TILE = 128u * 64u;  // bf16 outs of a warp of the epilogue: 128 tokens, 32 outputs
     static constexpr uint32_t ACCS = 2;
     static constexpr uint32_t EPI_WARPS = 8;
+    static constexpr uint32_t ASKER = 2u + EPI_WARPS;  // the second warp that asks for copies
     static constexpr uint32_t COLS = ACCS * TILE;
     static constexpr uint32_t OUT = RING;          // (without outs and residuals in shared memory: stages, too)
     static constexpr uint32_t FULL_BARS = OUT + EPI_WARPS * WARP_TILE;  // in the first block: both blocks' copies are there
@@ -667,13 +670,14 @@ __device__ __forceinline__ void mma_commit_pair(uint32_t bar, uint32_t first) {
 }
 
 template <bool E4M3>
-__global__ void __launch_bounds__(320, 1) linear_many_kernel(const __grid_constant__ LinearArgs a) {
+__global__ void __launch_bounds__(Many::THREADS, 1) linear_many_kernel(const __grid_constant__ LinearArgs a) {
     using S = Many;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t *smem = smem_raw + (base - smem_u32(smem_raw));
     volatile uint32_t *abort_word = reinterpret_cast<volatile uint32_t *>(smem + S::ABORT);
     const uint32_t tid = threadIdx.x, warp = __shfl_sync(FULL, tid / 32u, 0), lane = tid % 32u;
+    const bool epilogue = warp >= 2u && warp < S::ASKER;
     uint32_t in_cluster;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(in_cluster));
     const uint32_t rank = in_cluster & 1u, first = in_cluster & ~1u, share = in_cluster / 2u;
@@ -713,21 +717,28 @@ __global__ void __launch_bounds__(320, 1) linear_many_kernel(const __grid_consta
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (behind the allocation, as above)
 
-    if (warp == 0u) {
+    if (warp == 0u || warp >= S::ASKER) {
         if (lane == 0u) {
-            uint32_t i = 0, s = 0, phase = 0;  // steps so far; of the ring
+            const uint32_t which = warp == 0u ? 0u : warp - S::ASKER + 1u;
+            uint32_t i = 0, s = which, phase = 0;  // steps so far; of the ring
             bool gave_up = false;
             for (uint32_t tile = pair; tile < tiles && !gave_up; tile += pairs) {
                 const int32_t output0 = (int32_t)(tile / a.token_tiles * S::TILE + rank * TILE_M);
                 const int32_t token0 = (int32_t)(tile % a.token_tiles * a.tile_tokens + rank * (a.tile_tokens / 2u));
                 for (uint32_t k = from_step; k < to_step; ++k, ++i) {
+                    if (i % S::ASKERS != which) {
+                        continue;
+                    }
                     if (mbar_wait(base + S::EMPTY + 8 * s, phase ^ 1u, abort_word, a.wait_ns)) {
                         gave_up = true;
                         break;
                     }
                     const uint32_t bar = base + S::FULL_BARS + 8 * s, to = base + s * stage;
-                    s = s + 1u == stages ? 0u : s + 1u;
-                    phase ^= s == 0u;
+                    s += S::ASKERS;
+                    if (s >= stages) {
+                        s -= stages;
+                        phase ^= 1u;
+                    }
                     const int32_t x = (int32_t)(k * (E4M3 ? BLOCK_BYTES : BLOCK_BYTES / 2u));
                     if (i == a.lost_stage && blockIdx.x == 0u) {
                         continue;  // (test hook: the stage never fills)
@@ -785,7 +796,7 @@ __global__ void __launch_bounds__(320, 1) linear_many_kernel(const __grid_consta
             mbar_drain(base + S::FINAL, 0u, a.wait_ns);  // (nothing is freed under a multiply, on any way out)
         }
         __syncwarp();
-    } else if (warp >= 2u && a.shares == 1u) {
+    } else if (epilogue && a.shares == 1u) {
         const uint32_t quad = warp % 4u, half = (warp - 2u) / 4u;
         uint32_t turn = 0, loaded = 0;  // tiles; residuals asked for
         for (uint32_t tile = pair; tile < tiles; tile += pairs, ++turn) {
@@ -903,10 +914,10 @@ __global__ void __launch_bounds__(320, 1) linear_many_kernel(const __grid_consta
         const uint32_t mine = token0 + share * per + begin;  // this warp's tokens
         const uint32_t live = mine < a.tokens ? min(per / 2u, a.tokens - mine) : 0u;
         Output o = {1.0f, 0.0f, false};
-        const TokenScales scales(a, mine, warp >= 2u ? live : 0u);
+        const TokenScales scales(a, mine, epilogue ? live : 0u);
         float r[8];
         bool there = false;
-        if (warp >= 2u) {
+        if (epilogue) {
             o = output_of(a, n);
             residuals_of(a, o, mine, n, live, r);
             there = !warp_wait(base + S::ACC_FULL, 0u, abort_word, a.wait_ns);
@@ -1168,8 +1179,10 @@ extern "C" int32_t lily_linear(lily_sampler_t *h, void *stream_, const lily_line
                             (g.residual == nullptr || rows16(g.residual, g.residual_ld));
         // The tile's tokens and the shares of its columns, by the time of the busiest pair, in units of which 1900
         // are a microsecond. A step takes the longest of its multiplies (256 tokens 0.27 us), of what all pairs
-        // read (256 + t rows of 128 bytes each, 11.5 TB/s together), and of a copy's way (1.35 us) by the stages there
-        // are. A tile's end costs by its tokens (16 ns each), joining shares by the sums that are sent (two of 256 tokens 5 us).
+        // read (256 + t rows of 128 bytes each, 11.5 TB/s together), of a copy's way (1.35 us) by the stages there are, and of
+        // asking for its copies (0.18 us). A tile's end costs by its tokens (16 ns each), joining shares by the sums that
+        // are sent (two of 256 tokens 5 us). (512 x 4096 x 4096 e4m3, without the copies' way: tiles of 192 tokens for
+        // 128, 15.4 us for 13.0.)
         uint64_t most[3] = {};
         CU(h, e4m3 ? clusters_at_once<true>(most) : clusters_at_once<false>(most));
         const uint64_t pairs = most[0], output_tiles = (g.outputs + Many::TILE - 1ull) / Many::TILE;
@@ -1185,7 +1198,7 @@ extern "C" int32_t lily_linear(lily_sampler_t *h, void *stream_, const lily_line
                 }
                 const uint32_t stages = Many::stages_of(t, copies && shares == 1u);
                 const uint64_t steps = (tiles + pairs - 1u) / pairs * ((a.blocks + shares - 1u) / shares);
-                const uint64_t step = std::max<uint64_t>({2u * t, (256u + t) * std::min(tiles * shares, pairs) * 2u / 95u, 2565u / stages});
+                const uint64_t step = std::max<uint64_t>({2u * t, (256u + t) * std::min(tiles * shares, pairs) * 2u / 95u, 2565u / stages, 340u});
                 const uint64_t cost = steps * step + t / shares * 31u + (shares > 1u ? t * (shares - 1u) / shares * 70u + 1000u : 0u);
                 if (cost < best) {
                     best = cost;

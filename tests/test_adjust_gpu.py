@@ -418,3 +418,29 @@ def test_refusals(cuda, lily):
     empty = torch.zeros((2, 0), dtype=torch.int32, device="cuda")
     scratch.adjust_logits(logits, good, history_ids=empty, history_len=n)
     assert (logits == 0).all() and scratch.status() == lily.OK
+
+
+def test_misaligned_lists_are_refused(cuda, lily):
+    """By the host, before anything is enqueued."""
+    import ctypes as C
+
+    torch = cuda
+    scratch = lily.SamplerScratch(1000, max_rows=2)
+    logits, words = torch.zeros((2, 1000), device="cuda"), torch.zeros(4096, dtype=torch.int32, device="cuda")
+    device_params = torch.zeros(2 * C.sizeof(lily.SamplingParams) + 1, dtype=torch.uint8, device="cuda")
+    with pytest.raises(lily.LilyError) as e:
+        scratch.adjust_logits(logits, device_params[1:], params_on_device=True)
+    assert e.value.code == lily.ERR_ARG
+    fields = ("history_ids", "history_len", "bias_ids", "bias_vals", "bias_len", "ban_ids", "ban_len", "mask", "mask_rows",
+              "out_status")
+    for off in (None, *fields):
+        a = lily.AdjustArgs()
+        a.struct_size, a.rows = C.sizeof(lily.AdjustArgs), 2
+        a.logits = a.out = logits.data_ptr()
+        a.logits_ld = a.out_ld = 1000
+        for name in fields:
+            setattr(a, name, words.data_ptr() + (2 if name == off else 0))
+        a.history_ld = a.bias_ld = a.ban_ld = 4
+        a.mask_ld, a.masks = 32, 2
+        st = lily.lib().lily_adjust_logits(scratch._h, torch.cuda.current_stream().cuda_stream, C.byref(a))
+        assert st == (lily.OK if off is None else lily.ERR_ARG), off
