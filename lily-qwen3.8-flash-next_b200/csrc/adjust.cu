@@ -6,18 +6,18 @@
 //
 // Penalties and biases change a few thousand ids of a row, which the row's lists name: adjust_logits_kernel. A row
 // is cut into slices of the vocabulary (where there are few rows; a large batch's rows are a block each),
-// whose blocks' halves work side by side: the first passes over the slice's logits as above, the second
+// whose blocks' two parts work side by side: the first passes over the slice's logits as above, the second
 // marks the ids of the slice that the history has, a bit each, numbers them (a prefix sum over the bits), and
 // reads the history again to count them by their numbers: a few thousand counts instead of one for every
 // id. When both are done, the numbered ids, which lie evenly on the threads, are penalised. Blocks have nothing
 // to say to one another, so nothing is kept between calls and no workspace is needed.
 //
-// What bounds it: masks alone are a launch (1 x 151936 2.2 us on the device). 256 x 151936 bf16 to f32 with
-// histories of 32768 ids take 75 us where the bytes are 26: the history's half takes them (three reads of its ids, an
-// atomic in shared memory for each in two of them, scattered logits at the end), and a row is one block's, so
-// 256 of them fill 148 SMs unevenly. Slower there: counts of 16 bits for every id over four slices a row (116 us),
-// the rows' lists pulled by halves of a block (100), tasks in a pipeline (82 to 100), numbers handed out by
-// atomics that return (105).
+// What bounds it: masks alone are a launch (1 x 151936 2.2 us on the device). 256 x 151936 bf16 with histories of
+// 32768 ids take 58 us, 73 with masks, bans and biases, where the bytes are 26: the second part takes them (three reads
+// of the ids, an atomic in shared memory for each in two of them, scattered logits at the end), and a row is one
+// block's, so 256 of them fill 148 SMs unevenly. Slower there: counts of 16 bits for every id over four slices a row
+// (116 us for 75 at the time), the rows' lists pulled by halves of a block (100), tasks in a pipeline (82 to 100),
+// numbers handed out by atomics that return (105), parts whose threads go by the history's length (86 for 72: registers).
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -379,7 +379,8 @@ __global__ void __launch_bounds__(MASK_NT, 2) mask_logits_kernel(const __grid_co
     }
 }
 
-constexpr uint32_t NT = 512, HALF = NT / 2;
+constexpr uint32_t NT = 512;
+constexpr uint32_t LISTING = 320, STREAMING = NT - LISTING;  // threads of a block's two parts
 constexpr uint32_t WINDOW = 5120;  // numbered ids that a block counts at a time
 
 // Grid: rows x slices, the rows' first slices first.
@@ -404,27 +405,31 @@ __global__ void __launch_bounds__(NT, 2) adjust_logits_kernel(const __grid_const
     const uint32_t units = (task.n + shift + 31u) / 32u;  // words of bits
     const bool from_slot = task.from_slot(), history = task.history > 0u;
 
-    // The second half finds out what the lists say while the first one passes over the logits; where a
-    // short slice has a long history, both see to that together afterwards.
+    // The second part finds out what the lists say while the first one passes over the logits; where a
+    // short slice has a long history, both see to that together afterwards. (256 x 151936 bf16, the second part of
+    // 128, 192, 256, 320 and 384 threads: 32768 ids a row 105, 81, 65, 58 and 61 us; of 256, 320 and 384: 2048 ids 36,
+    // 39 and 48.) Without a history, both pass over the logits (16 biases and bans: 45 -> 36 us).
     const bool together = task.history > 2u * task.n;
-    if (t < HALF) {
-        task.stream(a, kept, t, HALF);
-    } else {
-        for (uint32_t i = t - HALF; history && i < (halves ? units * 16u : direct ? task.n + shift : units); i += HALF) {
+    const uint32_t streaming = history ? STREAMING : NT;
+    if (t < streaming) {
+        task.stream(a, kept, t, streaming);
+    }
+    if (t >= STREAMING) {
+        for (uint32_t i = t - STREAMING; history && i < (halves ? units * 16u : direct ? task.n + shift : units); i += LISTING) {
             (direct ? count_of : seen)[i] = 0u;
         }
-        for (uint32_t j = t - HALF; j < task.bias_len; j += HALF) {
+        for (uint32_t j = t - STREAMING; j < task.bias_len; j += LISTING) {
             bias_id[j] = __ldg(a.bias_ids + (uint64_t)task.row * a.bias_ld + j);
             bias_val[j] = __ldg(a.bias_vals + (uint64_t)task.row * a.bias_ld + j);
         }
-        if (t == HALF) {
+        if (t == STREAMING) {
             next_part = 0u;
         }
     }
     if (together) {
         __syncthreads();
     }
-    const uint32_t width = together ? NT : HALF, bar = together ? BAR_ALL : BAR_LISTS, me = together ? t : t - HALF;
+    const uint32_t width = together ? NT : LISTING, bar = together ? BAR_ALL : BAR_LISTS, me = together ? t : t - STREAMING;
     const HistoryList ids{a.history_ids + (uint64_t)task.row * a.history_ld, task.history, task.id0 - shift, shift, task.n};
     const auto mark_and_number = [&]() {
         ids.each(&next_part, [&](const uint32_t (&place)[8]) {
@@ -474,7 +479,7 @@ __global__ void __launch_bounds__(NT, 2) adjust_logits_kernel(const __grid_const
         }
         bar_sync(bar, width);
     };
-    if (history && (together || t >= HALF)) {
+    if (history && (together || t >= STREAMING)) {
         bar_sync(bar, width);
         // ---- the history's ids, a bit each (or their counts at once)
         if (direct) {
@@ -530,7 +535,7 @@ __global__ void __launch_bounds__(NT, 2) adjust_logits_kernel(const __grid_const
             });
         }
     };
-    if (history && !direct && (together || t >= HALF)) {
+    if (history && !direct && (together || t >= STREAMING)) {
         fill(0u, me, width, bar);
     }
     __syncthreads();  // (the logits are written, too)
