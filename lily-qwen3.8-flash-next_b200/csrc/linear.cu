@@ -661,7 +661,8 @@ __device__ __forceinline__ void mma_ss_pair(uint32_t d_tmem, uint64_t adesc, uin
     }
 }
 
-// Arrives at this barrier of both blocks of the pair, whose first in the cluster is `first`, once the multiplies issued so far have run.
+// Arrives at this barrier of both blocks of the pair, whose first in the cluster is `first`, once the multiplies
+// issued so far have run.
 __device__ __forceinline__ void mma_commit_pair(uint32_t bar, uint32_t first) {
     asm volatile(
         "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
@@ -965,6 +966,10 @@ __global__ void __launch_bounds__(Many::THREADS, 1) linear_many_kernel(const __g
         __syncwarp();
     }
 
+    if (rank == 1u && tid == 64u) {
+        mbar_drain(base + S::FINAL, 0u, a.wait_ns);  // (the last commit arrives in this block, too, before it ends)
+    }
+    __syncwarp();
     tc_fence_before();
     __syncthreads();
     cluster_arrive();
