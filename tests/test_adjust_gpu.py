@@ -444,3 +444,23 @@ def test_misaligned_lists_are_refused(cuda, lily):
         a.mask_ld, a.masks = 32, 2
         st = lily.lib().lily_adjust_logits(scratch._h, torch.cuda.current_stream().cuda_stream, C.byref(a))
         assert st == (lily.OK if off is None else lily.ERR_ARG), off
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_rows_beyond_32_bits(cuda, lily, bf16):
+    """Rows of logits more than 2^32 bytes apart; the last one is adjusted as it is alone."""
+    torch = cuda
+    rng = np.random.default_rng(77)
+    vocab, rows, pitch = 5001, 3, 2 ** 31 + 8
+    case = Case(rng, rows, vocab, bf16, history=300, lists=8, masks=2)
+    dtype = torch.bfloat16 if bf16 else torch.float32
+    buffer = torch.empty((rows - 1) * pitch + vocab, dtype=dtype, device="cuda")
+    far = buffer.as_strided((rows, vocab), (pitch, 1))
+    near = torch.from_numpy(case.logits).cuda().to(dtype)
+    far.copy_(near)
+    scratch = lily.SamplerScratch(vocab, max_rows=rows, max_history=512)
+    kw, params = case.args(torch, lily)
+    scratch.adjust_logits(near, params, **kw)
+    scratch.adjust_logits(far, params, **kw)
+    assert torch.equal(far, near)
+    assert scratch.status() == lily.OK

@@ -309,6 +309,23 @@ def test_a_wait_that_runs_out_is_reported(cuda, lily):
         _check(torch, out, a, w, kw)
 
 
+@pytest.mark.parametrize("tokens,pitch", [(3, 2 ** 31 + 8), (70, 2 ** 26), (70, 2 ** 26 + 1)])
+def test_offsets_beyond_32_bits(cuda, lily, tokens, pitch):
+    """Rows of a and out that lie more than 2^32 bytes apart in all; the residual is out itself."""
+    torch = cuda
+    g = torch.Generator(device="cuda").manual_seed(24)
+    scratch = _handle(lily)
+    buffer = torch.empty((tokens - 1) * pitch + 4096, dtype=torch.bfloat16, device="cuda")
+    a, w, kw = _inputs(torch, g, tokens, 256, 520, "bf16")
+    if pitch % 8 == 0:
+        a = buffer.as_strided((tokens, 256), (pitch, 1), 1024).copy_(a)
+    out = buffer.as_strided((tokens, 520), (pitch, 1))
+    residual = torch.randn((tokens, 520), generator=g, device="cuda").bfloat16()
+    out.copy_(residual)
+    scratch.linear(a, w, out, residual=out)
+    _check(torch, out, a, w, kw, residual=residual)
+
+
 def test_refusals(cuda, lily):
     torch = cuda
     scratch = _handle(lily)

@@ -208,3 +208,21 @@ def test_refusals(cuda, lily):
     scratch.clear_fault()
     scratch.add_rms_norm(x, w, out)
     assert scratch.status() == lily.OK
+
+
+@pytest.mark.parametrize("hidden,pitch", [(1000, 2 ** 31 + 8), (1001, 2 ** 31 + 3)])
+def test_rows_beyond_32_bits(cuda, lily, hidden, pitch):
+    """Rows more than 2^32 bytes apart, the sum in place: as rows that follow one another."""
+    torch = cuda
+    g = torch.Generator(device="cuda").manual_seed(hidden)
+    scratch = lily.SamplerScratch(64, max_rows=1, max_history=0)
+    x = torch.randn((3, hidden), generator=g, device="cuda").bfloat16()
+    residual = torch.randn((3, hidden), generator=g, device="cuda").bfloat16()
+    weight = torch.randn(hidden, generator=g, device="cuda")
+    want, total = torch.empty_like(x), torch.empty_like(x)
+    scratch.add_rms_norm(x, weight, want, residual=residual, residual_out=total)
+    buffer = torch.empty(2 * pitch + hidden, dtype=torch.bfloat16, device="cuda")
+    far = buffer.as_strided((3, hidden), (pitch, 1)).copy_(residual)
+    out = torch.empty_like(x)
+    scratch.add_rms_norm(x, weight, out, residual=far, residual_out=far)
+    assert torch.equal(out, want) and torch.equal(far, total)
