@@ -81,7 +81,7 @@ enum lily_activation {
  * lily_add_rms_norm writes them, and one per output). Products are summed on the tensor cores in
  * binary32, the epilogue is binary32, and `out` is rounded once.
  *
- * Any numbers of tokens, outputs and columns. The rows of a and weight start on 16-byte
+ * Any numbers of tokens, outputs and columns, up to 2^30 each. The rows of a and weight start on 16-byte
  * boundaries (their pitches multiples of 16 bytes); out, bias and residual need no alignment
  * beyond their elements'. `residual` may be `out` itself (the same address and pitch); else out
  * overlaps no other buffer. A call gives the same bits every time, and a token's do not depend

@@ -239,7 +239,7 @@ __device__ __forceinline__ uint32_t at_rank(uint32_t addr, uint32_t rank) {
 
 // ------------------------------------------------------------------ few tokens --
 //
-// Up to 64 tokens. Many tiles, of up to 128 outputs x N tokens: a block has one after the other, and finishes one
+// Up to 32 tokens, of bf16 heads up to 64. Many tiles, of up to 128 outputs x N tokens: a block has one after the other, and finishes one
 // while it multiplies the next; the tile's outputs are as many as give all blocks the same (1 x 4096 x 40000: with
 // 128 for 313 tiles on 296 blocks 60 us, with 72 51: 6.4 TB/s). Few: a cluster has one of 128, whose columns its blocks share out evenly. Each
 // sums its share in tensor memory, then sends every token's column of sums to the block that finishes that
@@ -257,16 +257,15 @@ struct Few {
     // Two blocks on an SM.
     static constexpr uint32_t MOST_STAGES = 10;
     static constexpr uint32_t RING = (N == 16u ? 5u : 4u) * (A_STAGE + B_STAGE);  // bytes of stages
-    // The sums that blocks send one another have a place of their own (a block may send as soon as the
-    // other runs), or, where that takes a stage, the stages' (it has to be done with its columns).
-    static constexpr bool OVER_STAGES = N >= 64u;
+    // The sums that blocks send one another have a place of their own: a block may send as soon as the other runs.
+    // (64 tokens come here with tiles for all blocks.)
+    static constexpr bool SHARES = N <= 32u;
     // Sums of successive steps go into accumulators in turn: shorter chains of additions. Two sets of them: a
     // tile is finished while the block's next one is multiplied.
     static constexpr uint32_t ACCS = 2, SETS = 2;
     static constexpr uint32_t COLS = SETS * ACCS * N;
-    static constexpr uint32_t PART = OVER_STAGES ? 0u : RING;
-    static constexpr uint32_t BARS = RING + (OVER_STAGES ? 0u : PART_BYTES);
-    static_assert(PART_BYTES <= RING, "room for the sums");
+    static constexpr uint32_t PART = RING;
+    static constexpr uint32_t BARS = RING + (SHARES ? PART_BYTES : 0u);
     static constexpr uint32_t EMPTY = BARS + 8u * MOST_STAGES;
     static constexpr uint32_t ACC_FULL = EMPTY + 8u * MOST_STAGES;
     static constexpr uint32_t ACC_EMPTY = ACC_FULL + 8u * SETS;
@@ -324,7 +323,7 @@ __global__ void __launch_bounds__(192) linear_few_kernel(const __grid_constant__
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(smem + S::TMEM_ADDR);
-    if (shares > 1u && !S::OVER_STAGES) {
+    if (S::SHARES && shares > 1u) {
         cluster_arrive();  // (this block has begun: the others may write into its shared memory)
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -431,7 +430,7 @@ __global__ void __launch_bounds__(192) linear_few_kernel(const __grid_constant__
             }
         }
     };
-    if (shares == 1u) {
+    if (!S::SHARES || shares == 1u) {
         uint32_t turn = 0;
         for (uint32_t tile = tile0; warp >= 2u && tile < tiles; tile += stride, ++turn) {
             const uint32_t b = turn % S::SETS, n = output_tile(tile) + row, live = a.tokens;
@@ -486,9 +485,6 @@ __global__ void __launch_bounds__(192) linear_few_kernel(const __grid_constant__
             tc_fence_after();
         }
         __syncwarp();
-        if (S::OVER_STAGES) {
-            cluster_arrive();
-        }
         cluster_wait();
         if (warp >= 2u) {
             for (uint32_t c = 0; c < live; c += 16u) {
@@ -577,7 +573,7 @@ __global__ void __launch_bounds__(192) linear_few_kernel(const __grid_constant__
 
 // ----------------------------------------------------------------- many tokens --
 //
-// From 65 tokens on. Tiles of 256 outputs x up to 256 tokens, each by a pair of blocks (a cluster of two on neighbouring
+// From 33 tokens on, of bf16 heads from 65. Tiles of 256 outputs x up to 256 tokens, each by a pair of blocks (a cluster of two on neighbouring
 // SMs) whose tensor cores multiply together: either block holds 128 outputs' weights and half of the tokens in
 // shared memory, and the pair's multiply reads both. That halves the bytes that a multiply takes
 // out of each SM's shared memory, which one block alone is bound by. The pairs stay for all of the launch; an
@@ -1084,9 +1080,9 @@ cudaError_t launch_many(const LinearArgs &a, uint32_t clusters, cudaStream_t str
 
 template <bool E4M3>
 cudaError_t few_by_tokens(const LinearArgs &a, uint32_t n, uint32_t blocks, uint32_t shares, cudaStream_t stream) {
-    return n == 16u   ? launch_few<16, E4M3>(a, blocks, shares, stream)
-           : n == 32u ? launch_few<32, E4M3>(a, blocks, shares, stream)
-                      : launch_few<64, E4M3>(a, blocks, shares, stream);
+    return n == 16u           ? launch_few<16, E4M3>(a, blocks, shares, stream)
+           : n == 32u || E4M3 ? launch_few<32, E4M3>(a, blocks, shares, stream)
+                              : launch_few<64, false>(a, blocks, shares, stream);
 }
 
 bool encode_rows(CUtensorMap *map, const void *p, uint64_t ld, uint32_t rows, uint32_t columns, uint32_t dtype,
@@ -1177,7 +1173,10 @@ extern "C" int32_t lily_linear(lily_sampler_t *h, void *stream_, const lily_line
 
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     const uint64_t sms = (uint32_t)h->sm_count;
-    if (g.tokens > 64u) {
+    // By pairs from 65 tokens on; from 33 unless the weights are bf16 and their tiles more than pairs (64 x 4096 x 11000:
+    // 20.7 us, by single blocks 23.0; 64 x 8192 x 2048 11.6 and 14.9; e4m3 33 x 2048 x 151936 53 and 67; the other way
+    // 64 x 2048 x 20000 21.3 and 19.9, 64 x 2048 x 151936 104 and 101).
+    if (g.tokens > 64u || (g.tokens > 32u && (e4m3 || (g.outputs + Many::TILE - 1ull) / Many::TILE <= sms / 2u))) {
         const auto rows16 = [&](const void *p, uint64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16u == 0u && ld * 2u % 16u == 0u; };
         // (A copy out of shared memory writes whole 16 bytes: rows of 1003 outputs had zeroes behind them.)
         const bool copies = !a.out_f32 && g.outputs % 8u == 0u && rows16(g.out, g.out_ld) &&
@@ -1227,14 +1226,13 @@ extern "C" int32_t lily_linear(lily_sampler_t *h, void *stream_, const lily_line
         return LILY_OK;
     }
     const uint32_t n = g.tokens <= 16u ? 16u : g.tokens <= 32u ? 32u : 64u;
-    // Shares of the columns: as many blocks as there are SMs, of four steps at least, of 64 tokens and bf16 eight
-    // (40 x 2048 x 2048: bf16, eight shares of four 8.8 us, four of eight 7.9; e4m3, four of four 6.3, two of eight
-    // 7.3); up to 32 tokens two on an SM, of eight (24 x 4096 x 4096: e4m3, four shares of eight steps 7.7 us, eight
-    // of four 8.2; bf16, of sixteen 10.6, of eight 9.4; 64 tokens on one block an SM 12.7 us, on two 14.1).
+    // Shares of the columns: as many blocks as there are SMs, of four steps at least; up to 32 tokens two on an SM, of
+    // eight (24 x 4096 x 4096: e4m3, four shares of eight steps 7.7 us, eight of four 8.2; bf16, of sixteen 10.6, of
+    // eight 9.4).
     uint64_t tiles = (g.outputs + TILE_M - 1ull) / TILE_M;
     uint32_t shares = 8u;
     while (shares > 1u && (tiles * shares > sms * (n <= 32u ? 2u : 1u) ||
-                           a.blocks < (tiles * shares > sms || (n > 32u && !e4m3) ? 8u : 4u) * shares)) {
+                           a.blocks < (tiles * shares > sms ? 8u : 4u) * shares)) {
         shares /= 2u;
     }
     // A tile's outputs, where blocks have tiles of their own: those of which the busiest block is done first. A step
