@@ -25,13 +25,15 @@ extern "C" {
  * The residual's addition and the root-mean-square norm, a token at a time:
  *
  *   h = x + residual                       (residual NULL: h = x)
- *   y = h / sqrt(mean(h^2) + eps) * (weight_offset + weight)
+ *   y = h * (weight_offset + weight) * (1 / sqrt(mean(h^2) + eps))
  *
- * h, its sum of squares and y are binary32; `residual_out` gets h rounded to `dtype`, the
+ * h, its sum of squares, both products (in this order) and y are binary32; `residual_out` gets h rounded to `dtype`, the
  * norm is taken of h as it is before that rounding. `out` is y rounded to F32 or BF16, or with
  * out_dtype LILY_E4M3 codes with one scale per token, y ~ code * scale:
  *
- *   m = max(|y|, 2^-64) over the token,  scale = m / 448,  code = e4m3(y * (448 / m)).
+ *   m = max(|y|, 2^-64) over the token,  scale = m / 448,  code = e4m3(y * (448 / m)),
+ *
+ * of the same binary32 y that an F32 out gets (rows that lie alike), a rounding a step.
  *
  * A NaN or an infinity makes its token's values what the formulas make of them, and no other's.
  *

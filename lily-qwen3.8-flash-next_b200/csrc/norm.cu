@@ -4,7 +4,7 @@
 // the residual are read once and h and out written once: 7 bytes a value with a bf16 residual and
 // 8-bit codes, and nothing else of size. One reduction serves both statistics: with u = h * weight,
 // y = u / rms, so the largest |y| is the largest |u| over rms, and the 8-bit codes need no
-// second round through the block.
+// second round through the block; they are those of y as the other types get it, rounded to binary32.
 //
 // What bounds it: memory from a few hundred tokens on (16384 x 4096 bf16 to codes 72 to 77 us with
 // its residual, 6.5 to 6.1 TB/s; 777 x 5001 f32 8.2 us, out of L2 in part); below, the launch and one way through a block:
@@ -302,21 +302,24 @@ __global__ void __launch_bounds__(WARPS ? 32u * WARPS : VECS == 1u ? 1024u : 512
             largest = __reduce_max_sync(0xFFFFFFFFu, lane < warps ? part_max[lane] : 0u);
         }
     }
-    float factor = 1.0f / sqrtf(fmaf(sum, a.inv_hidden, a.eps));
+    const float factor = 1.0f / sqrtf(fmaf(sum, a.inv_hidden, a.eps));
+    float to_codes = 1.0f;
     if (CODES) {
-        float m = __uint_as_float(largest) * factor;
-        m = m < 0x1p-64f ? 0x1p-64f : m;  // (a NaN stays)
+        float m = __uint_as_float(largest) * factor;  // (rounding keeps the order: this is the largest |y|, rounded)
+        m = m < 0x1p-64f ? 0x1p-64f : m;              // (a NaN stays)
         if (WARPS ? lane == 0u : t == 0u) {
             a.out_scales[token] = m / E4M3_MAX;
         }
-        factor *= E4M3_MAX / m;
+        to_codes = E4M3_MAX / m;
     }
     O *out = static_cast<O *>(a.out) + token * a.out_ld;
 #pragma unroll
     for (uint32_t j = 0; j < VECS; ++j) {
 #pragma unroll
         for (uint32_t k = 0; k < V; ++k) {
-            u[j][k] *= factor;
+            // (Not by factor * to_codes: that product rounds apart, 1e-5 of the codes came out beside those of y, and can
+            // pass the format's range where neither step does.)
+            u[j][k] = CODES ? u[j][k] * factor * to_codes : u[j][k] * factor;
         }
         store<O>(out, Vec(j, shift), n, u[j]);
     }
