@@ -54,7 +54,8 @@ enum lily_status {
 enum lily_row_status {
     LILY_ROW_OK = 0,
     LILY_ROW_NAN = 1,        /* a NaN among the adjusted logits */
-    LILY_ROW_NONFINITE = 2,  /* largest adjusted logit not finite (all banned) */
+    LILY_ROW_NONFINITE = 2,  /* largest adjusted logit not finite (all banned or masked); a greedy row
+                                without lists or penalties takes +inf, and never sees a NaN */
     LILY_ROW_PARAMS = 3,     /* device-resident params failed validation */
     LILY_ROW_LIST = 4,       /* history_len / bias_len / ban_len beyond max_history /
                                 max_list or beyond the list's row pitch: row refused */
@@ -343,7 +344,9 @@ int32_t lily_argmax_batch(lily_sampler_t *h, void *stream, const void *logits,
  * does to a row before it draws, for the paths whose draws take none of it (vocabulary shards,
  * the rows of a speculative step, a head of the caller's own), and masks by bits, which no
  * draw takes. Draw from the result with the penalties left out (lily_draft_params); a row then
- * draws what lily_sample_batch draws with everything in the call, as long as `out` is F32.
+ * draws what lily_sample_batch draws with everything in the call, as long as `out` is F32. (But for a
+ * greedy row with an infinity or a NaN: without lists of its own it takes the former and passes over the
+ * latter, with them it reports either.)
  *
  *   l = logit; for the row's bias entries of that id, in list order: l += value
  *   if penalties are on and count(id) > 0:
@@ -352,7 +355,8 @@ int32_t lily_argmax_batch(lily_sampler_t *h, void *stream, const void *logits,
  *   banned, or the id's bit in the row's mask is 0: l = -inf (whatever the logit was, NaN too)
  *
  * all in fp32, rounded once if `out` is BF16; the temperature stays with the draw. A row that
- * is left with nothing is all -inf, which the draw reports (LILY_ROW_NONFINITE).
+ * is left with nothing is all -inf, which the draw reports (LILY_ROW_NONFINITE), sampled or greedy, whole
+ * or merged from shards; lily_argmax_batch alone has an id for it.
  *
  * The logits are those of the ids [first_id, first_id + handle vocab): 0 for a whole row, a
  * shard's first id else. The ids of lists and masks are global; those outside the range have

@@ -116,16 +116,22 @@ static __global__ void __launch_bounds__(NT, 2) merge_rows_kernel(const __grid_c
         }
         return;
     }
-    if (in.flags & ROW_GREEDY) {  // (its best logit, whatever that is)
+    if (in.flags & ROW_GREEDY) {  // (its best logit, whatever that is, but -inf: see nothing_to_draw)
         if (lane == 0u) {
-            a.out_ids[row] = sm->id[0];
+            const bool none = sm->key[0] == key_of(neg_inf());
+            a.out_ids[row] = none ? 0xFFFFFFFFu : sm->id[0];
             if (a.out_status) {
-                a.out_status[row] = LILY_ROW_OK;
+                a.out_status[row] = none ? LILY_ROW_NONFINITE : LILY_ROW_OK;
             }
             if (a.kept_n) {
-                a.kept_n[row] = 1;
-                a.kept_ids[(uint64_t)row * a.kept_ld] = sm->id[0];
-                a.kept_probs[(uint64_t)row * a.kept_ld] = 1.0f;
+                a.kept_n[row] = none ? 0u : 1u;
+                if (!none) {
+                    a.kept_ids[(uint64_t)row * a.kept_ld] = sm->id[0];
+                    a.kept_probs[(uint64_t)row * a.kept_ld] = 1.0f;
+                }
+            }
+            if (none) {
+                atomicOr(a.status_word, 1u << LILY_ROW_NONFINITE);
             }
         }
         return;

@@ -770,6 +770,13 @@ __device__ __forceinline__ void pick(SmemFixed *sm, const float *cum, uint32_t n
     Team<SMALL>::sync();
 }
 
+// Whether a row whose best adjusted logit is `top` has nothing to draw: a sampled row needs a finite one. A greedy
+// row takes the largest there is, but no -inf: masks and bans leave those (an argmax by itself has a result for
+// every row).
+__device__ __forceinline__ bool nothing_to_draw(const RowCtx &c, const KArgs &a, float top) {
+    return c.argmax_mode ? top == neg_inf() && a.force_greedy == 0u : top == neg_inf() || top == -neg_inf();
+}
+
 // Steps 6-8 on the sorted candidates [0, n): softmax weights, sequential
 // prefix, cut, draw (plain or speculative), outputs.
 template <bool SMALL>
@@ -782,7 +789,7 @@ static __device__ __noinline__ void finalize(SmemFixed *sm, const KArgs &a, uint
     float *cum = reinterpret_cast<float *>(sm->tid);
     const float top = float_of_key(sm->key[0]);
     uint32_t err = sm->err;
-    if (!c.argmax_mode && err == 0 && (top == neg_inf() || top == -neg_inf())) {
+    if (err == 0 && nothing_to_draw(c, a, top)) {
         err = LILY_ROW_NONFINITE;
     }
     if (err != 0) {
@@ -956,7 +963,7 @@ static __device__ __noinline__ void finalize_warp(SmemFixed *sm, const KArgs &a,
     const uint32_t i0 = lane < n ? sm->id[lane] : 0xFFFFFFFFu, i1 = lane + 32u < n ? sm->id[lane + 32u] : 0xFFFFFFFFu;
     const float top = float_of_key(__shfl_sync(FULL, k0, 0));
     uint32_t err = sm->err;
-    if (!c.argmax_mode && err == 0 && (top == neg_inf() || top == -neg_inf())) {
+    if (err == 0 && nothing_to_draw(c, a, top)) {
         err = LILY_ROW_NONFINITE;
     }
     if (err != 0) {
@@ -1259,6 +1266,21 @@ __device__ __forceinline__ float frag_max<__nv_bfloat16>(const Frag &f) {
 
 __device__ __forceinline__ float widen(float x) { return x; }
 __device__ __forceinline__ float widen(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+// A NaN never wins a greedy row: it has the key of -inf. Where that is the best key, a NaN that stands for it gets
+// the least of all, so that rows of NaN alone are not taken for rows left with nothing. By one warp, before the
+// best becomes a draw or a shard's record.
+template <typename T>
+__device__ __forceinline__ void tell_nan_from_nothing(SmemFixed *sm, const T *row_ptr) {
+    if (sm->ctx.argmax_mode && sm->key[0] == key_of(neg_inf())) {
+        const float best = widen(row_ptr[sm->id[0]]);
+        __syncwarp();
+        if ((threadIdx.x & 31u) == 0u && best != best) {
+            sm->key[0] = 0u;
+        }
+        __syncwarp();
+    }
+}
 
 // Plain loads (any alignment) of the logits [base, base + GROUP) of a row;
 // slots at or past `hi` zero.
@@ -2721,13 +2743,14 @@ __device__ __forceinline__ void sample_row(const KArgs &a, const uint32_t row, c
             if (!sorted) {
                 sort_candidates<true>(sm, n);
             }
+            tell_nan_from_nothing(sm, row_ptr);
             ShardRecord *rec = a.cand_out + row;
             for (uint32_t i = tid; i < LILY_SHARD_CANDIDATES; i += 32u) {
                 rec->cand[i] = i < n ? make_uint2(sm->key[i], sm->id[i] + a.id_offset)
                                      : make_uint2(0u, 0xFFFFFFFFu);
             }
             if (tid == 0) {
-                rec->max_adj = float_of_key(sm->key[0]);
+                rec->max_adj = fmaxf(float_of_key(sm->key[0]), neg_inf());  // (of a NaN: -inf)
                 rec->sum_exp = 0.0f;
                 if (sm->err) {
                     atomicOr(a.status_word, 1u << (sm->err & 31u));
@@ -2742,6 +2765,7 @@ __device__ __forceinline__ void sample_row(const KArgs &a, const uint32_t row, c
             if (!sorted) {
                 sort_candidates<true>(sm, n);
             }
+            tell_nan_from_nothing(sm, row_ptr);
             LILY_STAMP(PH_SORT);
             if (row < a.spec.n_spec) {
                 finalize<true>(sm, a, row, n, P.seed);

@@ -768,12 +768,13 @@ __global__ void __launch_bounds__(NT, 2) stream_rows_kernel(const __grid_constan
             empty_record(sm->err ? sm->err : ROW_INTERNAL);
         } else if (tid < 32u) {
             // The sorted candidates are the row's record (ids in the whole vocabulary's numbering).
+            tell_nan_from_nothing(sm, row_ptr);
             ShardRecord *rec = a.cand_out + row;
             for (uint32_t i = tid; i < LILY_SHARD_CANDIDATES; i += 32u) {
                 rec->cand[i] = i < n ? make_uint2(sm->key[i], sm->id[i] + a.id_offset) : make_uint2(0u, 0xFFFFFFFFu);
             }
             if (tid == 0) {
-                rec->max_adj = float_of_key(sm->key[0]);
+                rec->max_adj = fmaxf(float_of_key(sm->key[0]), neg_inf());  // (of a NaN: -inf)
                 rec->sum_exp = total;
                 if (sm->err) {
                     atomicOr(a.status_word, 1u << (sm->err & 31u));
@@ -806,6 +807,7 @@ __global__ void __launch_bounds__(NT, 2) stream_rows_kernel(const __grid_constan
             sm->ctx.slot = table_mode ? slot : 0u;
         }
         __syncwarp();
+        tell_nan_from_nothing(sm, row_ptr);
         finalize_warp(sm, a, row, n, P.seed);
         if (stamps && tid == 0) {
             stamps[PH_END] = global_ns();

@@ -380,8 +380,12 @@ int lo_sample(const float *logits, uint32_t vocab, const lo_params_t *p,
         return LO_ERR_PARAMS;
     }
     if (lo_is_greedy(p) && !lo_uses_penalties(p) && n_bias == 0u && n_ban == 0u) {
-        /* src/kernels/sample.rs:382-385: not a sampled draw, the exact argmax. */
+        /* src/kernels/sample.rs:382-385: not a sampled draw, the exact argmax. A row of nothing but -inf
+         * (masked) has no draw. */
         *out_id = lo_argmax(logits, vocab);
+        if (logits[*out_id] == u2f(0xFF800000u)) {
+            return LO_ERR_NONFINITE;
+        }
         kept_ids[0] = *out_id;
         kept_w[0] = 1.0f;
         kept_cum[0] = 1.0f;
@@ -526,6 +530,10 @@ int lo_spec_verify(const float *target, uint32_t m, uint64_t ld, uint32_t vocab,
         uint32_t out;
         if (lo_is_greedy(p) && !pen) {
             out = lo_argmax(row, vocab);
+            if (row[out] == u2f(0xFF800000u)) {
+                status = status == LO_OK ? LO_ERR_NONFINITE : status;
+                out = 0xFFFFFFFFu;
+            }
         } else {
             uint32_t n_keep = 0, chosen = 0;
             int s = lo_sample(row, vocab, p, pen ? counts : NULL, NULL, NULL, 0, NULL, 0,
