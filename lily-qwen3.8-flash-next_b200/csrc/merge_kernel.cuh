@@ -80,7 +80,7 @@ static __global__ void __launch_bounds__(NT, 2) merge_rows_kernel(const __grid_c
                 const ShardRecord *rec = rec0 + (uint64_t)s * a.merge_stride;
                 sum += rec->sum_exp * expf(rec->max_adj - top);
             }
-            a.out_lse[row] = top + logf(sum);
+            a.out_lse[row] = top == neg_inf() ? top : top + logf(sum);  // (nothing is left: the logarithm of 0)
         }
         __syncthreads();
         n = sm->n;

@@ -146,3 +146,27 @@ def test_shards_of_tight_masks(cuda, lily, shards, rows):
                 greedy = p["temperature"] == 0.0 or p.get("top_k") == 1
                 exact = torch.logsumexp(scratch_rows.double() / (1.0 if greedy else p["temperature"]), 1)
                 assert (lse.double() - exact).abs().nan_to_num(0.0)[~torch.from_numpy(empty).cuda()].max() <= 2.0 ** -14
+
+
+@pytest.mark.parametrize("shards", [1, 2, 7])
+def test_the_sum_of_nothing(cuda, lily, shards):
+    """log 0 is -inf, from one shard's records and from several."""
+    import lily_b200.shard as sh
+
+    torch = cuda
+    part = lily.SamplerScratch(1000, max_rows=3)
+    for p in (dict(temperature=0.7, top_k=20), dict(temperature=0.0)):
+        params = [lily.SamplingParams(**p)] * 3
+        records = torch.empty((shards, 3, sh.RECORD_BYTES), dtype=torch.uint8, device="cuda")
+        for k in range(shards):
+            logits = torch.full((3, 1000), float("-inf"), device="cuda")
+            logits[1, 17] = 2.0 if k == shards - 1 else float("-inf")
+            part.shard_candidates(logits, params, records[k], first_id=1000 * k, want_sums=True)
+        out, status = (torch.full((3,), 77, dtype=torch.int32, device="cuda") for _ in range(2))
+        lse = torch.full((3,), 123.0, device="cuda")
+        part.merge_draw(records, params, out, uniforms=torch.zeros(3, device="cuda"), out_status=status, out_lse=lse)
+        assert part.status() == lily.ERR_DEVICE_ROW
+        assert status.tolist() == [lily.ROW_NONFINITE, 0, lily.ROW_NONFINITE]
+        assert np_u32(out).tolist() == [NONE, 1000 * (shards - 1) + 17, NONE]
+        assert torch.isneginf(lse[[0, 2]]).all(), lse
+        assert abs(float(lse[1]) - 2.0 / (p["temperature"] or 1.0)) <= 2.0 ** -14
