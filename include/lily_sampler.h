@@ -173,8 +173,8 @@ int32_t lily_sampler_status(lily_sampler_t *h, void *stream);
  * ends within the limit, all of a row's waits together within 1.75 of it.)
  *
  * inject_lost_copy is the device-side sibling of inject_fault, for tests: the
- * next LM-head launch on this handle (and only that one) leaves out the copy of
- * weight stage `stage` of its first block, so that the wait of the stage's
+ * next LM-head launch or product (lily_linear) on this handle, and only that one, leaves
+ * out the copy of weight stage `stage` of its first block, so that the wait of the stage's
  * consumers runs out. inject_lost_arrival likewise for the next draw: in each of its
  * clusters, block `block` waits for one arrival too many at one of its barriers (1 the
  * pool of keys, 2 the candidates, 3 the lists of a row that keeps many, 4 a shard's sums,

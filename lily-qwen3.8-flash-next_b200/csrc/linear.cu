@@ -582,6 +582,9 @@ __global__ void __launch_bounds__(192) linear_few_kernel(const __grid_constant__
 
     tc_fence_before();
     __syncthreads();
+    if (*abort_word) {
+        stay_for_landings();
+    }
     tc_fence_after();
     if (warp == 1u) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::COLS) : "memory");
@@ -765,12 +768,6 @@ __global__ void __launch_bounds__(Many::THREADS, 1) linear_many_kernel(const __g
                     }
                     tma_load_2d_pair(to, &a.w_map, at_rank(bar, first), x, output0);
                     tma_load_2d_pair(to + A_STAGE, &a.a_map, at_rank(bar, first), x, token0);
-                }
-            }
-            if (gave_up) {
-                // The copies asked for land in this block's shared memory, but are counted at the
-                // first block's barriers: this one stays for a millisecond, which no copy takes.
-                for (const uint64_t t0 = global_ns(); global_ns() - t0 < 1000000u;) {
                 }
             }
         }
@@ -990,6 +987,9 @@ __global__ void __launch_bounds__(Many::THREADS, 1) linear_many_kernel(const __g
     __syncthreads();
     cluster_arrive();
     cluster_wait();  // (neither block's barriers and tensor memory go while the other may use them)
+    if (*abort_word) {  // (a block's copies are counted at its pair's first block's barriers: that one has given up, too)
+        stay_for_landings();
+    }
     tc_fence_after();
     if (warp == 1u) {
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::COLS) : "memory");

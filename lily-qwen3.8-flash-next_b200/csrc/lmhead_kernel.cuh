@@ -799,6 +799,9 @@ __global__ void __launch_bounds__(Shape<N, FMT>::THREADS, 1) lmhead_kernel(const
 
     tc_fence_before();
     __syncthreads();
+    if (*abort_word) {
+        stay_for_landings();
+    }
     tc_fence_after();
     if (warp == 0u) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");

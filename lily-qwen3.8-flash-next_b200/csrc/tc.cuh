@@ -82,9 +82,10 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
 }
 
 // The same wait for the way out of a block that has given up: it does not look
-// at the abort word (which is set by then), only at its own clock. Used to let
-// copies and multiplies that are still in flight land before the block frees
-// its tensor memory and returns.
+// at the abort word (which is set by then), only at its own clock, and lasts up to
+// a millisecond, however short the limit is. Used to let copies and multiplies that are still in
+// flight land before the block frees its tensor memory and returns.
+constexpr uint64_t LANDING_NS = 1000000u;  // (no copy and no multiply takes that long)
 __device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity, uint64_t limit_ns) {
     const uint64_t t0 = global_ns();
     for (uint32_t spin = 0;; ++spin) {
@@ -96,9 +97,17 @@ __device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity, uint64
             : "=r"(done)
             : "r"(bar), "r"(parity)
             : "memory");
-        if (done || ((spin & 15u) == 15u && global_ns() - t0 > limit_ns)) {
+        if (done || ((spin & 15u) == 15u && global_ns() - t0 > max(limit_ns, LANDING_NS))) {
             return;
         }
+    }
+}
+
+// A block that has given up stays, when all of its threads are done, until nothing can be on its way into its
+// shared memory any more: a warp that asks for copies may have ended before another one gave up (a wait
+// limit of a few microseconds is shorter than a copy's way), and a pair's blocks arrive at each other's barriers.
+__device__ __forceinline__ void stay_for_landings() {
+    for (const uint64_t t0 = global_ns(); global_ns() - t0 < LANDING_NS;) {
     }
 }
 
