@@ -690,7 +690,9 @@ PyObject *py_adjust_logits(PyObject *, PyObject *const *v, Py_ssize_t n) {
         }
         if (PyObject *first = kw.get(N_FIRST_ID)) {
             a.first_id = word(first);
-            expect(PyLong_AsLongLong(first) == (long long)a.first_id);
+            const long long id = PyLong_AsLongLong(first);
+            PyErr_Clear();  // (-1 for what is larger: no error of this call's)
+            expect(id == (long long)a.first_id);
         }
         const Rows2 mask = rows_of(kw.get(N_MASK), device);
         if (mask.p != nullptr) {
