@@ -100,15 +100,16 @@ def sharded_lmhead_draw(scratch, weights, scales, hidden, params, out_ids, first
     import torch
 
     rows = hidden.shape[0]
-    if records is None:
-        records = torch.empty((rows, RECORD_BYTES), dtype=torch.uint8, device=hidden.device)
     on_stream = torch.cuda.stream(stream) if (stream is not None and hidden.is_cuda) else contextlib.nullcontext()
+    if records is None:
+        with on_stream:  # (the stream's own memory: free for others when its work is done)
+            records = torch.empty((rows, RECORD_BYTES), dtype=torch.uint8, device=hidden.device)
     if adjust is not None:
         import lily_b200 as lily
 
         with_penalties, params = params, [lily.draft_params(p) for p in params]
         if logits is None:
-            with on_stream:  # (the stream's own memory: free for others when its work is done)
+            with on_stream:
                 logits = torch.empty((rows, weights.shape[0]), device=hidden.device)
 
     def candidates():
