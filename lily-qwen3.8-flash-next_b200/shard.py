@@ -81,6 +81,14 @@ def gather_records(local_records, group=None):
     return out
 
 
+def _world(group, exchange) -> int:
+    import torch.distributed as dist
+
+    if exchange is not None:
+        return exchange.world
+    return dist.get_world_size(group) if dist.is_available() and dist.is_initialized() else 1
+
+
 def sharded_lmhead_draw(scratch, weights, scales, hidden, params, out_ids, first_id: int, *,
                         uniforms=None, steps=None, records=None, want_sums: bool = False,
                         out_lse=None, group=None, stream=None, exchange=None, adjust=None, logits=None, **kept):
@@ -92,8 +100,8 @@ def sharded_lmhead_draw(scratch, weights, scales, hidden, params, out_ids, first
     all-gather is the ranks' own stores into each other's memory instead.
 
     With `adjust`, a dict of keywords of SamplerScratch.adjust_logits (mask, history_ids,
-    bias_ids, ... by the whole vocabulary's ids, the same on every rank), the shard's logits
-    are written to `logits` (f32 [rows, shard], allocated if None), adjusted there with the penalties of
+    bias_ids, ... by the whole vocabulary's ids, the same on every rank; over several ranks no
+    count_slots, whose histograms are by a handle's own ids), the shard's logits are written to `logits` (f32 [rows, shard], allocated if None), adjusted there with the penalties of
     `params`, and drawn from without them."""
     import contextlib
 
@@ -107,6 +115,9 @@ def sharded_lmhead_draw(scratch, weights, scales, hidden, params, out_ids, first
     if adjust is not None:
         import lily_b200 as lily
 
+        # (The library refuses them for every shard but the first, which would wait for the others' records.)
+        if adjust.get("count_slots") is not None and _world(group, exchange) > 1:
+            raise lily.LilyError(lily.ERR_ARG, "count_slots: histograms know a shard's own ids only, give history_ids")
         with_penalties, params = params, [lily.draft_params(p) for p in params]
         if logits is None:
             with on_stream:
