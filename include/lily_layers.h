@@ -8,7 +8,8 @@
  * the caller owns every buffer, negative = refused on the host before anything was
  * enqueued, no CPU fallback. Any handle of the device serves (its fault latch, error
  * text, status word and wait limit; nothing else of it is used), and calls that overlap on
- * the GPU share nothing. All pointers are device pointers.
+ * the GPU share nothing. What they run is loaded when the device's first handle is made: a first call may
+ * be captured, and none allocates. All pointers are device pointers.
  */
 #ifndef LILY_LAYERS_H
 #define LILY_LAYERS_H
@@ -90,9 +91,6 @@ enum lily_activation {
  * on the tokens beside it; up to 64 tokens they do not depend on their number either as long as
  * that stays within 1..16, ..32 or ..64. (The columns are added up in shares whose number is
  * chosen by the sizes.)
- *
- * The first call of a kind loads its kernel (up to 16, 32, 64 tokens and more; BF16 or E4M3):
- * make it before a capture.
  */
 typedef struct lily_linear_args {
     uint32_t struct_size;    /* sizeof(lily_linear_args_t) */

@@ -369,8 +369,7 @@ int32_t lily_argmax_batch(lily_sampler_t *h, void *stream, const void *logits,
  * and the handle's sticky status. A row whose mask index is not below `masks` counts as LIST.
  *
  * Nothing of the handle is written but the status word: calls may overlap on the GPU. Masks
- * take ids up to 2^31 - 1 (LILY_ERR_CAPACITY beyond). The first call of a kind (masks and bans
- * alone, or any other list) loads its kernel: make it before a capture.
+ * take ids up to 2^31 - 1 (LILY_ERR_CAPACITY beyond).
  */
 typedef struct lily_adjust_args {
     uint32_t struct_size;        /* sizeof(lily_adjust_args_t) */

@@ -680,16 +680,7 @@ cudaError_t launch(Kernel kernel, const Launch &l, uint32_t blocks, uint32_t thr
 
 template <typename TI, typename TO, bool WIDE, uint32_t MAX_ROWS>
 cudaError_t launch_adjust(const AdjustLaunch<MAX_ROWS> &l, const Cut &cut, cudaStream_t stream) {
-    auto kernel = adjust_logits_kernel<TI, TO, WIDE, MAX_ROWS>;
-    static std::atomic<uint64_t> ready{0};  // (bit d: device d has seen the set-up)
-    int device = 0;
-    cudaError_t e = cudaGetDevice(&device);
-    const uint64_t bit = 1ull << (device & 63);
-    if (e == cudaSuccess && !(ready.load(std::memory_order_relaxed) & bit)) {
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)MOST_SMEM);
-        ready.fetch_or(e == cudaSuccess ? bit : 0u, std::memory_order_relaxed);
-    }
-    return e != cudaSuccess ? e : launch(kernel, l, l.a.tasks, NT, cut.smem, stream);
+    return launch(adjust_logits_kernel<TI, TO, WIDE, MAX_ROWS>, l, l.a.tasks, NT, cut.smem, stream);
 }
 
 template <typename TI, typename TO, uint32_t MAX_ROWS>
@@ -736,7 +727,34 @@ cudaError_t mask_rows(const AdjustArgs &a, const lily_adjust_args_t &g, uint32_t
 
 constexpr uint32_t ROWS_FEW = 16, ROWS_MANY = 256;
 
+// The variants that a call chooses from.
+template <typename TI, typename TO, bool WIDE>
+cudaError_t load_adjusts() {
+    for (const cudaError_t e : {load_kernel(mask_logits_kernel<TI, TO, WIDE>), load_kernel(adjust_logits_kernel<TI, TO, WIDE, 1>, MOST_SMEM),
+                                load_kernel(adjust_logits_kernel<TI, TO, WIDE, ROWS_FEW>, MOST_SMEM),
+                                load_kernel(adjust_logits_kernel<TI, TO, WIDE, ROWS_MANY>, MOST_SMEM)}) {
+        if (e != cudaSuccess) {
+            return e;
+        }
+    }
+    return cudaSuccess;
+}
+
 }  // namespace
+
+cudaError_t lily_host::adjust_ready() {
+    static std::atomic<uint64_t> seen{0};
+    return once_per_device(seen, [] {
+        using B = __nv_bfloat16;
+        for (const cudaError_t e : {load_adjusts<float, float, false>(), load_adjusts<float, float, true>(), load_adjusts<B, float, false>(),
+                                    load_adjusts<B, float, true>(), load_adjusts<B, B, false>(), load_adjusts<B, B, true>()}) {
+            if (e != cudaSuccess) {
+                return e;
+            }
+        }
+        return cudaSuccess;
+    });
+}
 
 extern "C" int32_t lily_adjust_logits(lily_sampler_t *h, void *stream_, const lily_adjust_args_t *args) {
     const int32_t st = check_handle(h);

@@ -336,8 +336,8 @@ int32_t launch(lily_sampler *h, cudaStream_t stream, const lily::KArgs &a, uint3
 // first call loads them.)
 cudaError_t load_kernels(const lily_sampler *h) {
     cudaError_t e = lily::split_ready(h->max_rows, (uint32_t)h->sm_count, h->max_smem);
-    if (e == cudaSuccess) {
-        e = lily::merge_ready();
+    for (auto ready : {lily::merge_ready, norm_ready, linear_ready, adjust_ready}) {
+        e = e == cudaSuccess ? ready() : e;
     }
     for (uint32_t log_blocks = 1; log_blocks <= 3u; ++log_blocks) {
         lily::split_rows_at_once(h->device, h->sm_count, h->max_smem, log_blocks);  // (asked of the device once)

@@ -6,6 +6,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <cmath>
 #include <string>
 #include <vector>
@@ -158,6 +159,33 @@ inline EncodeTiledFn tensor_map_encoder() {
         }
     }
     return fn;
+}
+
+// Every kernel that the norm, the product and the adjusted logits can come to, loaded on the current device (once;
+// norm.cu, linear.cu, adjust.cu).
+cudaError_t norm_ready();
+cudaError_t linear_ready();
+cudaError_t adjust_ready();
+
+// f() if the current device has not been through it before; `seen`: a bit for each.
+template <typename F>
+cudaError_t once_per_device(std::atomic<uint64_t> &seen, F f) {
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    const uint64_t bit = 1ull << (device & 63);
+    if (e == cudaSuccess && !(seen.load(std::memory_order_acquire) & bit)) {
+        e = f();
+        seen.fetch_or(e == cudaSuccess ? bit : 0u, std::memory_order_release);
+    }
+    return e;
+}
+
+// Loads a kernel; `smem`: its limit of dynamic shared memory, if that has to be raised.
+template <typename Kernel>
+cudaError_t load_kernel(Kernel kernel, uint32_t smem = 0) {
+    cudaFuncAttributes fa;
+    const cudaError_t e = cudaFuncGetAttributes(&fa, kernel);  // (this loads it)
+    return e != cudaSuccess || smem == 0u ? e : cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
 }
 
 }  // namespace lily_host

@@ -999,25 +999,8 @@ __global__ void __launch_bounds__(Many::THREADS, 1) linear_many_kernel(const __g
     }
 }
 
-template <typename Kernel>
-cudaError_t set_up(Kernel kernel, uint32_t bytes, std::atomic<uint64_t> &ready) {
-    int device = 0;
-    cudaError_t e = cudaGetDevice(&device);
-    const uint64_t bit = 1ull << (device & 63);  // (bit d: device d has seen the set-up)
-    if (e == cudaSuccess && !(ready.load(std::memory_order_relaxed) & bit)) {
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-        ready.fetch_or(e == cudaSuccess ? bit : 0u, std::memory_order_relaxed);
-    }
-    return e;
-}
-
 template <uint32_t N, bool E4M3>
 cudaError_t launch_few(const LinearArgs &a, uint32_t blocks, uint32_t shares, cudaStream_t stream) {
-    static std::atomic<uint64_t> ready{0};
-    const cudaError_t e = set_up(linear_few_kernel<N, E4M3>, Few<N>::BYTES, ready);
-    if (e != cudaSuccess) {
-        return e;
-    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(blocks, 1, 1);
     cfg.blockDim = dim3(Few<N>::THREADS, 1, 1);
@@ -1040,7 +1023,6 @@ cudaError_t launch_few(const LinearArgs &a, uint32_t blocks, uint32_t shares, cu
 // tiles: four shares 25.8 us, two 14.8).
 template <bool E4M3>
 cudaError_t clusters_at_once(uint64_t (&most)[3]) {
-    static std::atomic<uint64_t> ready{0};
     static std::atomic<uint32_t> known[64][3] = {};  // (plus one: 0 is not known)
     int device = 0;
     cudaError_t e = cudaGetDevice(&device);
@@ -1060,10 +1042,7 @@ cudaError_t clusters_at_once(uint64_t (&most)[3]) {
             cfg.attrs = attr;
             cfg.numAttrs = 1;
             int found = 0;
-            e = set_up(linear_many_kernel<E4M3>, Many::BYTES, ready);
-            if (e == cudaSuccess) {
-                e = cudaOccupancyMaxActiveClusters(&found, linear_many_kernel<E4M3>, &cfg);
-            }
+            e = cudaOccupancyMaxActiveClusters(&found, linear_many_kernel<E4M3>, &cfg);
             seen = (uint32_t)found + 1u;
             if (e == cudaSuccess) {
                 mine.store(seen, std::memory_order_relaxed);
@@ -1076,11 +1055,6 @@ cudaError_t clusters_at_once(uint64_t (&most)[3]) {
 
 template <bool E4M3>
 cudaError_t launch_many(const LinearArgs &a, uint32_t clusters, cudaStream_t stream) {
-    static std::atomic<uint64_t> ready{0};
-    const cudaError_t e = set_up(linear_many_kernel<E4M3>, Many::BYTES, ready);
-    if (e != cudaSuccess) {
-        return e;
-    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2u * a.shares * clusters, 1, 1);
     cfg.blockDim = dim3(Many::THREADS, 1, 1);
@@ -1131,6 +1105,23 @@ bool encode_outs(CUtensorMap *map, const void *p, uint64_t ld, const lily_linear
 }
 
 }  // namespace
+
+cudaError_t lily_host::linear_ready() {
+    static std::atomic<uint64_t> seen{0};
+    return once_per_device(seen, [] {
+        for (const cudaError_t e : {load_kernel(linear_few_kernel<16, false>, Few<16>::BYTES), load_kernel(linear_few_kernel<16, true>, Few<16>::BYTES),
+                                    load_kernel(linear_few_kernel<32, false>, Few<32>::BYTES), load_kernel(linear_few_kernel<32, true>, Few<32>::BYTES),
+                                    load_kernel(linear_few_kernel<64, false>, Few<64>::BYTES), load_kernel(linear_many_kernel<false>, Many::BYTES),
+                                    load_kernel(linear_many_kernel<true>, Many::BYTES)}) {
+            if (e != cudaSuccess) {
+                return e;
+            }
+        }
+        uint64_t most[3];
+        const cudaError_t e = clusters_at_once<false>(most);
+        return e != cudaSuccess ? e : clusters_at_once<true>(most);
+    });
+}
 
 extern "C" int32_t lily_linear(lily_sampler_t *h, void *stream_, const lily_linear_args_t *args) {
     const int32_t st = check_handle(h);

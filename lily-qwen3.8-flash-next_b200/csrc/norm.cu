@@ -325,6 +325,8 @@ __global__ void __launch_bounds__(WARPS ? 32u * WARPS : VECS == 1u ? 1024u : 512
     }
 }
 
+constexpr uint32_t NORM_WARPS = 8;  // of a block whose warps have a token each
+
 template <typename T, typename O, uint32_t VECS, Deal D, uint32_t WARPS>
 cudaError_t launch_norm(const NormArgs &a, cudaStream_t stream) {
     const uint32_t per = V * VECS, values = a.hidden + (D == SHIFTED ? V - 1u : 0u);
@@ -342,7 +344,7 @@ cudaError_t launch_norm(const NormArgs &a, cudaStream_t stream) {
 
 template <typename T, typename O>
 cudaError_t norm_by_size(const NormArgs &a, Deal deal, bool many, cudaStream_t stream) {
-    constexpr uint32_t WARPS = 8;
+    constexpr uint32_t WARPS = NORM_WARPS;
     if (deal == SCATTERED) {
         return a.hidden <= 8192u ? launch_norm<T, O, 1, SCATTERED, 0>(a, stream) : launch_norm<T, O, 8, SCATTERED, 0>(a, stream);
     }
@@ -378,6 +380,34 @@ cudaError_t norm_by_out(const NormArgs &a, uint32_t out_dtype, Deal deal, bool m
                                     : norm_by_size<T, __nv_fp8_e4m3>(a, deal, many, stream);
 }
 
+// The variants that norm_by_size chooses from.
+template <typename T, typename O>
+cudaError_t load_norms() {
+    constexpr uint32_t W = NORM_WARPS;
+    for (const cudaError_t e : {load_kernel(add_rms_norm_kernel<T, O, 1, SCATTERED, 0>), load_kernel(add_rms_norm_kernel<T, O, 8, SCATTERED, 0>),
+                                load_kernel(add_rms_norm_kernel<T, O, 1, ALIGNED, W>), load_kernel(add_rms_norm_kernel<T, O, 2, ALIGNED, W>),
+                                load_kernel(add_rms_norm_kernel<T, O, 4, ALIGNED, W>), load_kernel(add_rms_norm_kernel<T, O, 1, ALIGNED, 0>),
+                                load_kernel(add_rms_norm_kernel<T, O, 2, ALIGNED, 0>), load_kernel(add_rms_norm_kernel<T, O, 4, ALIGNED, 0>),
+                                load_kernel(add_rms_norm_kernel<T, O, 8, ALIGNED, 0>), load_kernel(add_rms_norm_kernel<T, O, 1, SHIFTED, 0>),
+                                load_kernel(add_rms_norm_kernel<T, O, 2, SHIFTED, 0>), load_kernel(add_rms_norm_kernel<T, O, 4, SHIFTED, 0>),
+                                load_kernel(add_rms_norm_kernel<T, O, 8, SHIFTED, 0>)}) {
+        if (e != cudaSuccess) {
+            return e;
+        }
+    }
+    return cudaSuccess;
+}
+
+template <typename T>
+cudaError_t load_norms_of() {
+    for (const cudaError_t e : {load_norms<T, float>(), load_norms<T, __nv_bfloat16>(), load_norms<T, __nv_fp8_e4m3>()}) {
+        if (e != cudaSuccess) {
+            return e;
+        }
+    }
+    return cudaSuccess;
+}
+
 uint32_t element(uint32_t dtype) { return dtype == LILY_F32 ? 4u : dtype == LILY_BF16 ? 2u : 1u; }
 
 // Whether rows of `ld` elements all start on multiples of `bytes`.
@@ -387,6 +417,14 @@ bool rows_at(const void *p, uint64_t ld, uint32_t dtype, uint32_t rows, uint32_t
 }
 
 }  // namespace
+
+cudaError_t lily_host::norm_ready() {
+    static std::atomic<uint64_t> seen{0};
+    return once_per_device(seen, [] {
+        const cudaError_t e = load_norms_of<float>();
+        return e != cudaSuccess ? e : load_norms_of<__nv_bfloat16>();
+    });
+}
 
 extern "C" int32_t lily_add_rms_norm(lily_sampler_t *h, void *stream, const lily_norm_args_t *args) {
     const int32_t st = check_handle(h);
