@@ -2394,7 +2394,6 @@ __device__ __forceinline__ void sample_row(const KArgs &a, const uint32_t row, c
 
     // ---- C'. pass 2 of the two-pass route: the fixed threshold, no meetings
     if (lean) {
-        const uint32_t n_lists = min(sm->n, CAP);  // what the lists pushed
         const float c_fix = sm->c_raw;
         {
             uint32_t base = c.lo + tid * GROUP;
@@ -2418,10 +2417,11 @@ __device__ __forceinline__ void sample_row(const KArgs &a, const uint32_t row, c
         }
         if (__syncthreads_or(*reinterpret_cast<volatile uint32_t *>(&sm->overflow))) {
             // More logits tie with the threshold than the buffer holds: start the
-            // stream over on the general path, which makes room as it goes.
+            // stream over on the general path, which makes room as it goes. What the lists pushed stays: n_adj
+            // entries. (Not sm->n as it was when this thread came to the pass: others may have pushed by then, and
+            // their raw logits passed for keys.)
             if (tid == 0) {
-                sm->n = n_lists;
-                sm->n_adj = n_lists;
+                sm->n = sm->n_adj;
                 sm->overflow = 0;
                 sm->ckey = sm->key;
                 sm->cid = sm->id;
