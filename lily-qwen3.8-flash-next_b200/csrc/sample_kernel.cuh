@@ -2482,6 +2482,7 @@ __device__ __forceinline__ void sample_row(const KArgs &a, const uint32_t row, c
             atomicAdd(&sm->cnt, (uint32_t)__popc(dropped));
             __syncthreads();
             const bool at_once = sm->n + sm->cnt <= CAP;
+            __syncthreads();  // (all of them have read the count: from here on it grows)
             for (uint32_t b = 0; b < 32u; ++b) {
                 const bool mine = (dropped >> b) & 1u;
                 if (!at_once) {

@@ -6,7 +6,8 @@ import pytest
 pytestmark = pytest.mark.gpu
 
 
-@pytest.mark.parametrize("rows,vocab,dtype", [(592, 4608, "float32"), (600, 8700, "bfloat16"), (300, 20_000, "float32"), (271, 4964, "float32")])
+@pytest.mark.parametrize("rows,vocab,dtype", [(592, 4608, "float32"), (600, 8700, "bfloat16"), (300, 20_000, "float32"), (271, 4964, "float32"),
+                                              (271, 7696, "float32"), (300, 8100, "float32"), (300, 11_000, "float32")])
 def test_rows_of_ties_again_and_again(cuda, lily, rows, vocab, dtype):
     import lily_b200.shard as sh
 
