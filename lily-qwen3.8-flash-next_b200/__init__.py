@@ -464,7 +464,7 @@ class SamplerScratch:
         self._check(lib().lily_sampler_set_wait_limit(self._h, nanoseconds))
 
     def inject_lost_copy(self, stage: int):
-        """Test hook: the next LM-head launch leaves out one weight copy of its first block."""
+        """Test hook: the next LM-head launch or product leaves out one weight copy of its first block."""
         lib().lily_sampler_inject_lost_copy(self._h, stage)
 
     def inject_lost_arrival(self, barrier: int, block: int):
